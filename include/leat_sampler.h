@@ -276,6 +276,98 @@ int leat_shard_select(leat_shard_t* shard, const leat_sample_args* args, leat_st
 int leat_shard_finish(leat_shard_t* shard, const leat_sample_args* args, leat_stream_t stream);
 int leat_shard_result(leat_shard_t* shard, const leat_sample_args* args, leat_stream_t stream);
 
+/* Beam search (no reference counterpart: leat decodes one sequence per request).  A step is one
+   leat_beam_select and one leat_reorder_states; leat_beam_sequences reads the answer back.  These
+   entries and leat_token_logprobs take no handle: all they need is in their arguments, the scratch
+   is the caller's for the call (any 256-byte aligned memory, its contents of no account before and
+   after), and calls that overlap on different streams share nothing unless they are given the same
+   scratch or outputs.
+
+   leat_beam_select: of each group's beams' continuations, the `width` best.  A live beam k with score
+   s continues with every token t whose logit x_t is above -inf, to the score s + x_t - lse, lse = ln
+   of the row's sum of exp(x) (a NaN logit counts as -inf, a +inf one as the largest float).  A
+   finished beam continues with end_id alone, its score unchanged.  A beam whose score is not finite
+   is dead and continues with nothing.  The logits of finished and dead beams are not read.
+   Continuations are ranked by score / ((5 + length) / 6)^length_penalty, where length is the
+   beam's, plus one for a live beam; equal ranks by the lower beam, then the larger logit, then the
+   lower token.  Scores and ranks are held in double precision; out_scores is rounded once.  Where a
+   group has fewer than `width` continuations the rest read: token -1, score -inf, not finished,
+   length 0, and as parent the beam of the place itself (place % beams). */
+typedef struct leat_beam_args {
+  const void* logits; /* (groups * beams, vocab): float32, or as LEAT_FLAG_LOGITS_BF16 / _F16 say */
+  int32_t groups;
+  int32_t beams;      /* 1..64 */
+  int32_t vocab;
+  int32_t width;      /* 1..64 */
+  int64_t row_stride; /* in logits */
+  uint32_t flags;     /* LEAT_FLAG_LOGITS_BF16 or LEAT_FLAG_LOGITS_F16 or 0 */
+  int32_t end_id;     /* -1: beams do not finish */
+  const float* scores;     /* (groups, beams) */
+  const uint8_t* finished; /* (groups, beams) bytes, non-zero where finished; or NULL: none */
+  const int32_t* lengths;  /* (groups, beams) tokens so far; or NULL, with length_penalty 0 */
+  float length_penalty;    /* -16..16; 0: by score alone */
+  int32_t* out_tokens;     /* (groups, width), best first */
+  int32_t* out_parents;    /* (groups, width) the beam each continues, 0..beams-1 */
+  float* out_scores;       /* (groups, width) */
+  uint8_t* out_finished;   /* (groups, width) or NULL: the token is end_id */
+  int32_t* out_lengths;    /* (groups, width) or NULL; needs lengths */
+  void* workspace;
+  size_t workspace_bytes;  /* at least leat_beam_workspace_bytes(groups * beams, vocab, width) */
+} leat_beam_args;
+
+/* Scratch of leat_beam_select, and of leat_token_logprobs with width = top (0..64); 0 for sizes that
+   are out of range. */
+size_t leat_beam_workspace_bytes(int32_t rows, int32_t vocab, int32_t width);
+int leat_beam_select(const leat_beam_args* args, leat_stream_t stream);
+
+/* Per-beam state that follows its beam, in place: for every tensor, row(g, k) takes what
+   row(g, parents[g, k]) held before the call, in the places [start, end) of each of its `outer` runs;
+   everything else stays as it is.  row(g, k) is slots[g, k], or g * beams + k when slots is NULL.
+   Parents outside 0..beams-1 and slots outside 0..rows-1 leave their rows alone.  The slots of a call
+   are distinct, and rows do not overlap.  start / end: (groups) on the device, or NULL for start_all /
+   end_all; cut to 0..places. */
+typedef struct leat_state {
+  void* data;
+  int64_t row_stride;   /* bytes from one row to the next */
+  int64_t outer_stride; /* bytes from one run of places to the next */
+  int64_t place_bytes;  /* bytes of one place; the places of a run lie back to back */
+  int32_t outer;        /* runs per row (heads that lie outside the places; 1 otherwise) */
+  int32_t places;       /* places per run (1 for a state without places) */
+  int32_t rows;
+} leat_state;
+int leat_reorder_states(const leat_state* states, int32_t count, const int32_t* parents, const int32_t* slots,
+                        int32_t groups, int32_t beams, const int32_t* start, int32_t start_all,
+                        const int32_t* end, int32_t end_all, leat_stream_t stream);
+
+/* What the steps of a search add up to: tokens and parents (steps, groups, beams) as every step's
+   leat_beam_select left them -> out_tokens (groups, beams, steps), the tokens of each beam of the last
+   step from the first step on, and out_lengths (groups, beams).  With end_id >= 0 a sequence's length
+   ends with its first end_id, and only end_id stands behind it; -1: none.  Before a parent outside
+   0..beams-1 the tokens read -1.  beams 1..64. */
+int leat_beam_sequences(const int32_t* tokens, const int32_t* parents, int32_t steps, int32_t groups, int32_t beams,
+                        int32_t end_id, int32_t* out_tokens, int32_t* out_lengths, leat_stream_t stream);
+
+/* Log-probabilities, as a server reports them beside its tokens (no reference counterpart): of the
+   given ids, and of each row's `top` likeliest tokens with their ids, the lower id first among equal
+   logits.  x_t - lse as for leat_beam_select.  Ids outside 0..vocab-1 read -inf; where a row has fewer
+   than `top` logits above -inf the rest read -inf with id -1. */
+typedef struct leat_logprob_args {
+  const void* logits; /* (rows, vocab): float32, or as LEAT_FLAG_LOGITS_BF16 / _F16 say */
+  int32_t rows;
+  int32_t vocab;
+  int64_t row_stride; /* in logits */
+  uint32_t flags;
+  int32_t given;      /* ids per row, 0 and up */
+  int32_t top;        /* 0..64 */
+  const int32_t* ids; /* (rows, given) */
+  float* out_logprobs;     /* (rows, given) */
+  float* out_top_logprobs; /* (rows, top) */
+  int32_t* out_top_ids;    /* (rows, top) */
+  void* workspace;
+  size_t workspace_bytes;  /* at least leat_beam_workspace_bytes(rows, vocab, top) */
+} leat_logprob_args;
+int leat_token_logprobs(const leat_logprob_args* args, leat_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

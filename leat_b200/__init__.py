@@ -8,6 +8,8 @@ _LAZY = {
     "Sampling": "sampler", "GREEDY": "sampler", "sample": "sampler", "Sampler": "sampler",
     "Sampled": "sampler", "default_sampler": "sampler", "ops": None, "speculative": None,
     "sharded": None, "workloads": None, "history": None, "SlotHistory": "history",
+    "beam": None, "BeamSearch": "beam", "beam_select": "beam", "reorder_states": "beam", "beam_sequences": "beam",
+    "logprobs": None, "token_logprobs": "logprobs",
 }  # fmt: skip
 
 

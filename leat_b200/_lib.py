@@ -31,6 +31,7 @@ EXPORTS = [
     "leat_candidate_record_bytes", "leat_candidate_record_layout", "leat_sample_from_records",
     "leat_shard_region_bytes", "leat_peer_alloc", "leat_peer_open", "leat_peer_close", "leat_peer_free",
     "leat_shard_create", "leat_shard_destroy", "leat_shard_select", "leat_shard_finish", "leat_shard_result",
+    "leat_beam_workspace_bytes", "leat_beam_select", "leat_reorder_states", "leat_beam_sequences", "leat_token_logprobs",
 ]  # fmt: skip
 
 
@@ -51,6 +52,39 @@ class SampleArgs(C.Structure):
         ("out_kept", C.c_void_p), ("out_probs", C.c_void_p), ("out_prob_ids", C.c_void_p),
         ("out_width", C.c_int32), ("status", C.c_void_p),
         ("softcap", C.c_float), ("position_scalar", C.c_int32),
+    ]  # fmt: skip
+
+
+class BeamArgs(C.Structure):
+    """struct leat_beam_args"""
+
+    _fields_ = [
+        ("logits", C.c_void_p), ("groups", C.c_int32), ("beams", C.c_int32), ("vocab", C.c_int32), ("width", C.c_int32),
+        ("row_stride", C.c_int64), ("flags", C.c_uint32), ("end_id", C.c_int32),
+        ("scores", C.c_void_p), ("finished", C.c_void_p), ("lengths", C.c_void_p), ("length_penalty", C.c_float),
+        ("out_tokens", C.c_void_p), ("out_parents", C.c_void_p), ("out_scores", C.c_void_p),
+        ("out_finished", C.c_void_p), ("out_lengths", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]  # fmt: skip
+
+
+class State(C.Structure):
+    """struct leat_state"""
+
+    _fields_ = [
+        ("data", C.c_void_p), ("row_stride", C.c_int64), ("outer_stride", C.c_int64), ("place_bytes", C.c_int64),
+        ("outer", C.c_int32), ("places", C.c_int32), ("rows", C.c_int32),
+    ]  # fmt: skip
+
+
+class LogprobArgs(C.Structure):
+    """struct leat_logprob_args"""
+
+    _fields_ = [
+        ("logits", C.c_void_p), ("rows", C.c_int32), ("vocab", C.c_int32), ("row_stride", C.c_int64), ("flags", C.c_uint32),
+        ("given", C.c_int32), ("top", C.c_int32), ("ids", C.c_void_p),
+        ("out_logprobs", C.c_void_p), ("out_top_logprobs", C.c_void_p), ("out_top_ids", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]  # fmt: skip
 
 
@@ -101,9 +135,15 @@ def _load() -> C.CDLL:
     lib.leat_shard_select.argtypes = [p, C.POINTER(SampleArgs), p]
     lib.leat_shard_finish.argtypes = [p, C.POINTER(SampleArgs), p]
     lib.leat_shard_result.argtypes = [p, C.POINTER(SampleArgs), p]
+    lib.leat_beam_workspace_bytes.restype = sz
+    lib.leat_beam_workspace_bytes.argtypes = [i32, i32, i32]
+    lib.leat_beam_select.argtypes = [C.POINTER(BeamArgs), p]
+    lib.leat_reorder_states.argtypes = [C.POINTER(State), i32, p, p, i32, i32, p, i32, p, i32, p]
+    lib.leat_beam_sequences.argtypes = [p, p, i32, i32, i32, i32, p, p, p]
+    lib.leat_token_logprobs.argtypes = [C.POINTER(LogprobArgs), p]
     for name in EXPORTS:
         fn = getattr(lib, name)
-        if name not in ("leat_sampler_workspace_bytes", "leat_sampler_last_cuda_error", "leat_candidate_record_bytes",
+        if name not in ("leat_sampler_workspace_bytes", "leat_beam_workspace_bytes", "leat_sampler_last_cuda_error", "leat_candidate_record_bytes",
                         "leat_shard_region_bytes"):
             fn.restype = C.c_int
     return lib

@@ -1,0 +1,330 @@
+"""Beam search on the device: the selection over beams and vocabulary, the caches and other states that
+follow their beams, and the sequences read back at the end.  leat decodes one sequence per request; this
+serves requests that ask for the best of several.
+
+`BeamSearch` runs a batch of searches step by step; `beam_select`, `reorder_states` and
+`beam_sequences` are its parts.  Nothing here waits for the device or copies to the host, and a call's
+scratch is its own, so every part can be captured into a CUDA graph."""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from leat_b200 import _lib
+from leat_b200.logprobs import FORMATS, launch, rows_of_logits, scratch
+
+MAX_BEAMS = 64
+MAX_WIDTH = 64
+
+
+@dataclass
+class Selected:
+    """The continuations of a step, (G, width) each, best first."""
+
+    tokens: torch.Tensor  # int32; -1 where a group has no further continuation
+    parents: torch.Tensor  # int32: the beam of the group that each continues
+    scores: torch.Tensor  # float32: summed log-probabilities; -inf where there is none
+    finished: torch.Tensor | None = None  # bool: the sequence has ended (with end_id)
+    lengths: torch.Tensor | None = None  # int32: tokens so far, the end token included (with lengths)
+
+
+@dataclass
+class Sequences:
+    tokens: torch.Tensor  # (G, K, T) int32
+    lengths: torch.Tensor  # (G, K) int32: tokens up to the first end token, which is included
+
+
+def _whole(x, dtype, shape, device, name: str) -> torch.Tensor:
+    if not isinstance(x, torch.Tensor) or x.dtype != dtype or x.device != device or tuple(x.shape) != shape:
+        raise ValueError(f"{name} must be a {shape} {str(dtype).removeprefix('torch.')} tensor on {device}")
+    return x if x.is_contiguous() else x.contiguous()
+
+
+def beam_select(logits, scores: torch.Tensor, width: int | None = None, *, finished: torch.Tensor | None = None,
+                end_id: int | None = None, lengths: torch.Tensor | None = None, length_penalty: float = 0.0,
+                out: Selected | None = None) -> Selected:  # fmt: skip
+    """The `width` (1..64, default K) best continuations of each of G groups of K beams (up to 64).
+
+    logits (G * K, V) float32, bfloat16 or float16, row g * K + k for beam k of group g; scores (G, K)
+    float32, what each beam's tokens add up to.  A beam continues with any token whose logit is above
+    -inf, to its score plus the token's log-probability; a beam of score -inf (or NaN) is dead and
+    continues with nothing (the first step of a search has one live beam per group, the others dead).
+    With `end_id`, a beam marked in `finished` (G, K) bool goes on as itself: one continuation, end_id,
+    its score unchanged; its logits are not read.  With `lengths` (G, K) int32, continuations are ranked
+    by score / ((5 + length) / 6) ** length_penalty (Wu et al. 2016) over their own lengths.  Equal
+    ranks: the lower beam, then the larger logit, then the lower token.  Ranks are held in 64 bits.
+
+    Masks are the caller's: set a forbidden token's logit to -inf (or the type's lowest value, which
+    makes it the last resort).  A row with nothing left has no continuations; a group with too few of
+    them has tokens of -1 and scores of -inf in the last places, with their own place as parent.
+    `out`: a Selected of an earlier call (or of your own contiguous tensors) to write into."""
+    logits = rows_of_logits(logits)
+    dev = logits.device
+    rows, vocab = logits.shape
+    if not isinstance(scores, torch.Tensor) or scores.dim() != 2:
+        raise ValueError("scores must be a (G, K) float32 tensor")
+    groups, beams = scores.shape
+    scores = _whole(scores, torch.float32, (groups, beams), dev, "scores")
+    if not 1 <= beams <= MAX_BEAMS or groups * beams != rows:
+        raise ValueError(f"logits must have a row per beam of scores (G, K), K from 1 to {MAX_BEAMS}")
+    width = beams if width is None else width
+    if isinstance(width, bool) or not isinstance(width, int) or not 1 <= width <= MAX_WIDTH:
+        raise ValueError(f"width must be an integer from 1 to {MAX_WIDTH}")
+    if end_id is not None and (isinstance(end_id, bool) or not isinstance(end_id, int) or not 0 <= end_id < vocab):
+        raise ValueError("end_id must be a token of the vocabulary")
+    if finished is not None:
+        if end_id is None:
+            raise ValueError("finished beams continue with end_id: give one")
+        finished = _whole(finished, torch.bool, (groups, beams), dev, "finished")
+    if lengths is not None:
+        lengths = _whole(lengths, torch.int32, (groups, beams), dev, "lengths")
+    elif length_penalty != 0.0:
+        raise ValueError("length_penalty needs the beams' lengths")
+    if not -16.0 <= length_penalty <= 16.0:
+        raise ValueError("length_penalty must be a number from -16 to 16")
+    shape = (groups, width)
+    if out is None:
+        tokens, parents, bits, *more = torch.empty((3 if lengths is None else 4, groups, width), dtype=torch.int32, device=dev).unbind(0)
+        out = Selected(tokens, parents, bits.view(torch.float32))
+        if lengths is not None:
+            out.lengths = more[0]
+        if end_id is not None:
+            out.finished = torch.empty(shape, dtype=torch.bool, device=dev)
+    else:
+        wanted = [(out.tokens, torch.int32), (out.parents, torch.int32), (out.scores, torch.float32)]
+        wanted += [(out.finished, torch.bool)] if end_id is not None else []
+        wanted += [(out.lengths, torch.int32)] if lengths is not None else []
+        for t, dtype in wanted:
+            if t is None or t.dtype != dtype or tuple(t.shape) != shape or t.device != dev or not t.is_contiguous():
+                raise ValueError(f"out must hold contiguous {shape} tensors on {dev}, of the types of a Selected")
+            if t.numel() and t.data_ptr() in (x.data_ptr() for x in (scores, finished, lengths) if x is not None):
+                raise ValueError("out must not be what the step reads")
+    if groups == 0:
+        return out
+    held, at, size = scratch(rows, vocab, width, dev)
+    a = _lib.BeamArgs(
+        logits.data_ptr(), groups, beams, vocab, width, logits.stride(0), FORMATS[logits.dtype], -1 if end_id is None else end_id,
+        scores.data_ptr(), None if finished is None else finished.data_ptr(), None if lengths is None else lengths.data_ptr(),
+        length_penalty, out.tokens.data_ptr(), out.parents.data_ptr(), out.scores.data_ptr(),
+        None if end_id is None else out.finished.data_ptr(), None if lengths is None else out.lengths.data_ptr(), at, size)  # fmt: skip
+    launch(dev, "leat_beam_select", _lib.lib.leat_beam_select, a)
+    return out
+
+
+def _state(t: torch.Tensor, dim: int | None) -> tuple:
+    """A tensor as leat_state has it: rows, runs of places per row, places, and their strides in bytes."""
+    shape, stride, size = t.shape, t.stride(), t.element_size()
+    if dim is None:
+        if t.dim() == 1:
+            return (t.data_ptr(), stride[0] * size, 0, size, 1, 1, shape[0])
+        dim = 1
+        places_are_all = True
+    else:
+        places_are_all = False
+    # a place is everything behind `dim`, a run its places: both must lie back to back
+    inner = 1
+    for i in range(t.dim() - 1, dim, -1):
+        if shape[i] != 1 and stride[i] != inner:
+            raise ValueError("the dimensions behind the places' must be contiguous")
+        inner *= shape[i]
+    places = shape[dim]
+    if places > 1 and stride[dim] != inner:
+        raise ValueError("places must lie back to back")
+    # the dimensions between the rows' and the places' make one run after another of one stride
+    outer, outer_stride = 1, 0
+    for i in range(dim - 1, 0, -1):
+        if shape[i] == 1:
+            continue
+        if outer == 1:
+            outer_stride = stride[i]
+        elif stride[i] != outer_stride * outer:
+            raise ValueError("the dimensions between rows and places must have one common stride")
+        outer *= shape[i]
+    if places_are_all:
+        inner, places = inner * places, 1
+    return (t.data_ptr(), stride[0] * size, outer_stride * size, inner * size, outer, places, shape[0])
+
+
+def _overlaps(row_stride: int, outer_stride: int, place_bytes: int, outer: int, places: int, rows: int) -> bool:
+    run = place_bytes * places
+    if rows < 2:
+        return outer > 1 and outer_stride < run
+    if outer < 2:
+        return row_stride < run
+    rows_outside = outer_stride >= run and row_stride >= outer_stride * (outer - 1) + run
+    rows_inside = row_stride >= run and outer_stride >= row_stride * (rows - 1) + run
+    return not (rows_outside or rows_inside)
+
+
+def _range_end(x, groups: int, device, name: str):
+    """A bound of the places: (pointer or None, value for all groups, tensor to keep)."""
+    if isinstance(x, torch.Tensor):
+        x = _whole(x, torch.int32, (groups,), device, name)
+        return x.data_ptr(), 0, x
+    if isinstance(x, bool) or not isinstance(x, int) or x < 0:
+        raise ValueError(f"{name} must be a number of places, or a ({groups},) int32 tensor of them")
+    return None, min(x, 0x7FFFFFFF), None
+
+
+def reorder_states(states, parents: torch.Tensor, *, slots: torch.Tensor | None = None, dim: int | None = None,
+                   start=0, length=None) -> None:  # fmt: skip
+    """Makes per-beam states follow their beams, in place: in every tensor of `states`, the row of beam k
+    of group g takes what the row of beam parents[g, k] held.  Rows that keep their place are not touched.
+
+    states: a tensor or a list of them, of any type, rows first; row g * K + k belongs to beam k of group
+    g, or row slots[g, k] where `slots` (G, K) int32 is given (cache slots; all different).  parents (G, K)
+    int32, K up to 64, as beam_select returns them.
+
+    `dim`: the dimension that counts positions, the same in every tensor (a cache (rows, heads,
+    positions, size) has 2, a cache (rows, positions, heads, size) has 1); then only positions `start`
+    to `length` follow, each an int or a (G,) int32 tensor on the device: positions before `start` (a
+    prompt that the beams share) and from `length` on stay as they are.  The places of a row, and what
+    lies behind `dim`, must be back to back.  Without `dim` whole rows follow.
+
+    Parents outside 0..K-1 and slots outside the tensor leave their row as it is."""
+    states = [states] if isinstance(states, torch.Tensor) else list(states)
+    if not isinstance(parents, torch.Tensor) or parents.dim() != 2 or not parents.is_cuda:
+        raise ValueError("parents must be a (G, K) int32 CUDA tensor")
+    groups, beams = parents.shape
+    dev = parents.device
+    parents = _whole(parents, torch.int32, (groups, beams), dev, "parents")
+    if not 1 <= beams <= MAX_BEAMS or groups > 65535:
+        raise ValueError(f"parents must be (G, K) with K from 1 to {MAX_BEAMS} and G up to 65535")
+    if slots is not None:
+        slots = _whole(slots, torch.int32, (groups, beams), dev, "slots")
+    if dim is None and (length is not None or (start is not None and not (isinstance(start, int) and start == 0))):
+        raise ValueError("start and length count positions: say which dimension they are with dim")
+    start_at, start_all, keep_start = _range_end(0 if start is None else start, groups, dev, "start")
+    end_at, end_all, keep_end = _range_end(0x7FFFFFFF if length is None else length, groups, dev, "length")
+    described = []
+    for t in states:
+        if not isinstance(t, torch.Tensor) or t.device != dev or t.dim() == 0 or t.layout != torch.strided or t.requires_grad:
+            raise ValueError(f"states must be tensors on {dev}, rows first, that need no gradient")
+        if slots is None and t.shape[0] < groups * beams:
+            raise ValueError("states must have a row per beam, or slots must say which rows are the beams'")
+        if dim is not None and not 0 < dim < t.dim():
+            raise ValueError("dim must be a dimension of every state, behind the rows'")
+        if t.numel() == 0:
+            continue
+        s = _state(t, dim)
+        if _overlaps(*s[1:]):
+            raise ValueError("the rows of a state must not overlap")
+        described.append(s)
+    if not described or groups == 0:
+        return
+    array = (_lib.State * len(described))(*described)
+    launch(dev, "leat_reorder_states", _lib.lib.leat_reorder_states, array, len(described), parents.data_ptr(),
+           None if slots is None else slots.data_ptr(), groups, beams, start_at, start_all, end_at, end_all)  # fmt: skip
+    del keep_start, keep_end
+
+
+def beam_sequences(tokens: torch.Tensor, parents: torch.Tensor, end_id: int | None = None) -> Sequences:
+    """The sequences of the last step's beams: tokens and parents (T, G, K) int32, a step's beam_select
+    results (width K) one behind the other -> tokens (G, K, T) and lengths (G, K).  With `end_id` a
+    sequence's length ends with its first end token, and only end tokens stand behind it."""
+    if not isinstance(tokens, torch.Tensor) or tokens.dim() != 3 or not tokens.is_cuda:
+        raise ValueError("tokens must be a (T, G, K) int32 CUDA tensor")
+    steps, groups, beams = tokens.shape
+    dev = tokens.device
+    tokens = _whole(tokens, torch.int32, (steps, groups, beams), dev, "tokens")
+    parents = _whole(parents, torch.int32, (steps, groups, beams), dev, "parents")
+    if not 1 <= beams <= MAX_BEAMS:
+        raise ValueError(f"there must be 1 to {MAX_BEAMS} beams")
+    if end_id is not None and (isinstance(end_id, bool) or not isinstance(end_id, int) or not 0 <= end_id <= 0x7FFFFFFF):
+        raise ValueError("end_id must be a token")
+    out = Sequences(torch.empty((groups, beams, steps), dtype=torch.int32, device=dev),
+                    torch.empty((groups, beams), dtype=torch.int32, device=dev))  # fmt: skip
+    if groups:
+        launch(dev, "leat_beam_sequences", _lib.lib.leat_beam_sequences, tokens.data_ptr(), parents.data_ptr(), steps, groups, beams,
+               -1 if end_id is None else end_id, out.tokens.data_ptr(), out.lengths.data_ptr())  # fmt: skip
+    return out
+
+
+class BeamSearch:
+    """G searches of K beams, step by step, up to `max_steps` tokens each, on one device and stream.
+
+        search = BeamSearch(groups, beams, max_steps, end_id=end, length_penalty=0.6, device=device)
+        for position in range(prompt, prompt + max_steps):
+            logits = model(tokens, caches, position)              # (G * K, V)
+            tokens = search.step(logits, caches, dim=2, start=prompt, length=position + 1)
+        best = search.sequences()                                 # tokens (G, K, T), best beam first
+
+    A step selects the beams' continuations, makes `states` follow their beams (reorder_states), and
+    returns the tokens the beams run next."""
+
+    def __init__(self, groups: int, beams: int, max_steps: int, *, end_id: int | None = None, length_penalty: float = 0.0, device=None):
+        if groups <= 0 or not 1 <= beams <= MAX_BEAMS or max_steps <= 0:
+            raise ValueError(f"groups and max_steps must be positive, beams from 1 to {MAX_BEAMS}")
+        self.groups, self.beams, self.max_steps = groups, beams, max_steps
+        self.end_id, self.length_penalty = end_id, length_penalty
+        self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        self._tokens = torch.empty((max_steps, groups, beams), dtype=torch.int32, device=self.device)
+        self._parents = torch.empty((max_steps, groups, beams), dtype=torch.int32, device=self.device)
+        # what a step reads and what it writes, in turn
+        make = lambda: (torch.empty((groups, beams), dtype=torch.float32, device=self.device),  # noqa: E731
+                        torch.zeros((groups, beams), dtype=torch.bool, device=self.device),
+                        torch.zeros((groups, beams), dtype=torch.int32, device=self.device))  # fmt: skip
+        self._beams = [make(), make()]
+        self.steps = 0
+        self.reset()
+
+    def reset(self) -> None:
+        """New searches: one live beam per group."""
+        scores, finished, lengths = self._beams[0]
+        scores.fill_(float("-inf"))
+        scores[:, 0] = 0.0
+        finished.zero_()
+        lengths.zero_()
+        self.steps = 0
+
+    @property
+    def scores(self) -> torch.Tensor:
+        """(G, K) float32 summed log-probabilities of the beams, best rank first."""
+        return self._beams[self.steps & 1][0]
+
+    @property
+    def finished(self) -> torch.Tensor:
+        """(G, K) bool"""
+        return self._beams[self.steps & 1][1]
+
+    @property
+    def lengths(self) -> torch.Tensor:
+        """(G, K) int32"""
+        return self._beams[self.steps & 1][2]
+
+    @property
+    def parents(self) -> torch.Tensor:
+        """(G, K) int32: the beams that the last step's beams continue."""
+        if self.steps == 0:
+            raise ValueError("no step has been taken")
+        return self._parents[self.steps - 1]
+
+    def step(self, logits, states=(), *, slots: torch.Tensor | None = None, dim: int | None = None, start=0, length=None,
+             history=None) -> torch.Tensor:  # fmt: skip
+        """One token for every beam: logits (G * K, V) of the beams' last tokens -> tokens (G * K, 1) int32
+        to run next (0 for beams that are dead: a group with fewer continuations than beams).  `states`
+        follow their beams as reorder_states says, and `history` (a SlotHistory whose slots `slots` are
+        the beams') does too and takes the tokens."""
+        if self.steps >= self.max_steps:
+            raise ValueError(f"the search was made for {self.max_steps} steps")
+        if history is not None and slots is None:
+            raise ValueError("history needs the beams' slots")
+        (scores, finished, lengths), (new_scores, new_finished, new_lengths) = self._beams[self.steps & 1], self._beams[1 - (self.steps & 1)]
+        out = Selected(self._tokens[self.steps], self._parents[self.steps], new_scores, new_finished, new_lengths)
+        ends = self.end_id is not None
+        beam_select(logits, scores, finished=finished if ends else None, end_id=self.end_id, lengths=lengths,
+                    length_penalty=self.length_penalty, out=out)  # fmt: skip
+        states = [states] if isinstance(states, torch.Tensor) else list(states)
+        if states:
+            reorder_states(states, out.parents, slots=slots, dim=dim, start=start, length=length)
+        if history is not None:
+            history.reorder(slots, out.parents)
+            history.append(slots, out.tokens)
+        self.steps += 1
+        return out.tokens.clamp(min=0).reshape(-1, 1)
+
+    def sequences(self) -> Sequences:
+        """The tokens of the steps so far, of every beam."""
+        return beam_sequences(self._tokens[: self.steps], self._parents[: self.steps], self.end_id)

@@ -10,9 +10,11 @@ from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent / "csrc"
 LIBRARY = CSRC / "libleat_sampler.so"
-SOURCES = [CSRC / "leat_sampler.cu"]
+SOURCES = [CSRC / "leat_sampler.cu", CSRC / "leat_beam.cu"]
 HEADERS = [CSRC / "sampler_kernels.cuh", CSRC / "device_util.cuh", CSRC / "stream_ring.cuh",
-           CSRC / "general_kernel.cuh", CSRC / "filter_path.cuh",
+           CSRC / "general_kernel.cuh", CSRC / "filter_path.cuh", CSRC / "finish_list.cuh",
+           CSRC / "argmax_kernel.cuh", CSRC / "shard_exchange.cuh", CSRC / "host_util.cuh",
+           CSRC / "beam_tiles.cuh", CSRC / "beam_merge.cuh", CSRC / "reorder_kernel.cuh", CSRC / "sequences_kernel.cuh",
            CSRC.parent.parent / "include" / "leat_sampler.h"]  # fmt: skip
 # -fmad=false: the CPU statement of the algorithm rounds every product and sum separately, and
 # ids must match it bit for bit

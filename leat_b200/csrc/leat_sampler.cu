@@ -11,6 +11,7 @@
 #include <mutex>
 #include <new>
 
+#include "host_util.cuh"
 #include "sampler_kernels.cuh"
 
 using namespace leat;
@@ -27,11 +28,15 @@ constexpr int kFilterMinVocab = 16384;  // narrower rows are not worth three lau
 
 thread_local char g_cuda_error[256] = "";
 
-int cuda_failed(cudaError_t e, const char* what) {
+}  // namespace
+
+int leat::cuda_failed(cudaError_t e, const char* what) {
   if (e == cudaSuccess) return 0;
   snprintf(g_cuda_error, sizeof(g_cuda_error), "%s: %s", what, cudaGetErrorString(e));
   return 1;
 }
+
+namespace {
 
 int round_up(int x, int m) { return (x + m - 1) / m * m; }
 int next_pow2(int x) { int p = 1; while (p < x) p <<= 1; return p; }
@@ -175,8 +180,6 @@ size_t lean_shared(int vocab, int history_cap, bool has_history, int old_ht_size
   return total > redo ? total : redo;
 }
 
-bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
-
 int check_broadcast(const void* p, int n, int rows) { return !p || n == rows || n == 1; }
 
 int fill_params(const leat_sampler* h, const leat_sample_args* a, KParams& P) {
@@ -229,25 +232,6 @@ int pick_vec(const KParams& P) {
   bool ok = P.vocab % per_vec == 0 && P.row_stride % per_vec == 0 && aligned(P.logits, 16);
   if (P.seen) ok = ok && P.seen_stride % 4 == 0 && aligned(P.seen, 4);
   return ok ? 4 : 1;
-}
-
-// A launch that may begin while the kernel before it in the stream still runs (programmatic
-// dependent launch); the kernel itself waits, with grid_dependency_wait(), before it reads what
-// that kernel writes.
-template <typename... Params, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t shared, cudaStream_t stream,
-                             Args... args) {
-  cudaLaunchConfig_t config = {};
-  config.gridDim = grid;
-  config.blockDim = block;
-  config.dynamicSmemBytes = shared;
-  config.stream = stream;
-  cudaLaunchAttribute attribute[1];
-  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute[0].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attribute;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
 template <bool PEN>

@@ -55,6 +55,22 @@ class SlotHistory:
         self.ids[slots, place] = torch.where(keep, tokens.to(torch.int32), old)
         self.count[slots] = (count + keep.to(torch.long)).to(torch.int32)
 
+    def reorder(self, slots: torch.Tensor, parents: torch.Tensor) -> None:
+        """A step of beam search: slots (G, K) are the beams' slots, and slot (g, k) takes the tokens that
+        slot (g, parents[g, k]) had (leat_b200.beam.reorder_states)."""
+        slots, parents = slots.to(self.device, torch.int32), parents.to(self.device, torch.int32)
+        if slots.dim() != 2 or slots.shape != parents.shape:
+            raise ValueError("slots and parents must be (G, K)")
+        if self.ids.is_cuda:
+            from leat_b200.beam import reorder_states
+
+            reorder_states([self.ids, self.count], parents, slots=slots)
+            return
+        known = (parents >= 0) & (parents < parents.shape[1])
+        own = torch.arange(parents.shape[1]).expand_as(parents)
+        to, of = slots.long().reshape(-1), slots.long().gather(1, torch.where(known, parents.long(), own)).reshape(-1)
+        self.ids[to], self.count[to] = self.ids[of], self.count[of]
+
     def rows(self, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """(history, history_len) for a decode step over `slots`: what sample() takes."""
         slots = slots.to(self.device, torch.long).reshape(-1)

@@ -1,0 +1,92 @@
+"""Log-probabilities of tokens under rows of logits, as a server reports them beside what it sampled and
+as a score of a prompt: of given ids, and of each row's likeliest tokens.  One pass over the logits,
+no handle, no host synchronisation; scratch is allocated per call on the current stream."""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from leat_b200 import _lib
+from leat_b200.sampler import device_tensor
+
+FORMATS = {torch.float32: 0, torch.bfloat16: _lib.FLAG_LOGITS_BF16, torch.float16: _lib.FLAG_LOGITS_F16}
+MAX_TOP = 64
+
+
+@dataclass
+class TokenLogprobs:
+    logprobs: torch.Tensor | None  # (B, M) float32: of the given ids
+    top_logprobs: torch.Tensor | None = None  # (B, top) float32, likeliest first, -inf-padded
+    top_ids: torch.Tensor | None = None  # (B, top) int32, the lower id first among equals, -1-padded
+
+
+def rows_of_logits(logits) -> torch.Tensor:
+    """`logits` as the kernels take it: (B, V) on the device, adjacent logits adjacent in memory."""
+    logits = device_tensor(logits)
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in FORMATS or not logits.is_cuda:
+        raise ValueError("logits must be a (B, V) float32, bfloat16 or float16 CUDA tensor")
+    if logits.shape[1] == 0:
+        raise ValueError("logits must have at least one token per row")
+    if (logits.stride(1) != 1 and logits.shape[1] > 1) or (logits.stride(0) < logits.shape[1] and logits.shape[0] > 1):
+        logits = logits.contiguous()
+    return logits
+
+
+def scratch(rows: int, vocab: int, width: int, device) -> tuple[torch.Tensor, int, int]:
+    """A call's workspace: the tensor that holds it, its 256-byte aligned address and its size.  It is
+    the call's own (the caching allocator keeps it for the current stream), so calls on several
+    streams or in several graphs share nothing."""
+    size = _lib.lib.leat_beam_workspace_bytes(rows, vocab, width)
+    held = torch.empty(size + 256, dtype=torch.uint8, device=device)
+    return held, (held.data_ptr() + 255) & ~255, size
+
+
+def launch(device: torch.device, what: str, call, *args) -> None:
+    """call(*args, stream) on `device` and its current stream."""
+    if torch.cuda.current_device() == device.index:
+        code = call(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            code = call(*args, torch.cuda.current_stream().cuda_stream)
+    if code != _lib.OK:
+        _lib.check(code, what)
+
+
+def token_logprobs(logits, ids=None, top: int = 0) -> TokenLogprobs:
+    """Log-probabilities under softmax(logits): of `ids` (B,) or (B, M) (int32 or int64, on the device),
+    and of each row's `top` likeliest tokens (0..64), with their ids.  logits (B, V) float32, bfloat16
+    or float16.  Results are float32, (B, M) and (B, top).
+
+    A NaN logit counts as -inf.  Ids outside the vocabulary (a -1 of padding) and tokens of logit -inf
+    have log-probability -inf, as does everything in a row without a logit above -inf."""
+    logits = rows_of_logits(logits)
+    rows, vocab = logits.shape
+    dev = logits.device
+    if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= MAX_TOP:
+        raise ValueError(f"top must be an integer from 0 to {MAX_TOP}")
+    given = 0
+    if ids is not None:
+        ids = device_tensor(ids)
+        if ids.dtype not in (torch.int32, torch.int64) or ids.device != dev:
+            raise ValueError("ids must be an int32 or int64 tensor on the logits' device")
+        if ids.dim() not in (1, 2) or ids.shape[0] != rows:
+            raise ValueError("ids must be (B,) or (B, M), a row per row of logits")
+        if ids.dtype == torch.int64:  # (what does not fit 32 bits is outside every vocabulary)
+            ids = ids.clamp(-1, vocab).to(torch.int32)
+        ids = ids.reshape(rows, -1 if rows else (ids.shape[1] if ids.dim() == 2 else 1)).contiguous()
+        given = ids.shape[1]
+    out = TokenLogprobs(torch.empty((rows, given), dtype=torch.float32, device=dev) if ids is not None else None)
+    if top:
+        out.top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=dev)
+        out.top_ids = torch.empty((rows, top), dtype=torch.int32, device=dev)
+    if rows == 0 or given + top == 0:
+        return out
+    held, at, size = scratch(rows, vocab, top, dev)
+    a = _lib.LogprobArgs(
+        logits.data_ptr(), rows, vocab, logits.stride(0), FORMATS[logits.dtype], given, top, ids.data_ptr() if given else None,
+        out.logprobs.data_ptr() if given else None, out.top_logprobs.data_ptr() if top else None,
+        out.top_ids.data_ptr() if top else None, at, size)  # fmt: skip
+    launch(dev, "leat_token_logprobs", _lib.lib.leat_token_logprobs, a)
+    return out
