@@ -305,7 +305,7 @@ typedef struct leat_beam_args {
   const float* scores;     /* (groups, beams) */
   const uint8_t* finished; /* (groups, beams) bytes, non-zero where finished; or NULL: none */
   const int32_t* lengths;  /* (groups, beams) tokens so far; or NULL, with length_penalty 0 */
-  float length_penalty;    /* -16..16; 0: by score alone */
+  float length_penalty;    /* -4..4; 0: by score alone */
   int32_t* out_tokens;     /* (groups, width), best first */
   int32_t* out_parents;    /* (groups, width) the beam each continues, 0..beams-1 */
   float* out_scores;       /* (groups, width) */

@@ -82,8 +82,8 @@ def beam_select(logits, scores: torch.Tensor, width: int | None = None, *, finis
         lengths = _whole(lengths, torch.int32, (groups, beams), dev, "lengths")
     elif length_penalty != 0.0:
         raise ValueError("length_penalty needs the beams' lengths")
-    if not -16.0 <= length_penalty <= 16.0:
-        raise ValueError("length_penalty must be a number from -16 to 16")
+    if not -4.0 <= length_penalty <= 4.0:
+        raise ValueError("length_penalty must be a number from -4 to 4")
     shape = (groups, width)
     if out is None:
         tokens, parents, bits, *more = torch.empty((3 if lengths is None else 4, groups, width), dtype=torch.int32, device=dev).unbind(0)

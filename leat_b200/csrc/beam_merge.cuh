@@ -1,17 +1,24 @@
-// From the tiles' headers and candidates (beam_tiles.cuh) to answers: a group's best continuations,
-// or a row's log-probabilities.
+// From the tiles' headers and their chunks' maxima (beam_tiles.cuh) to answers: a group's best
+// continuations, or a row's log-probabilities.
 //
 // A continuation (beam k, token t) has score_k + x_t - lse_k and is ranked by that over its length's
 // penalty.  Sums, scores and ranks are held in 64 bits: what is compared differs between beams by
 // their lse, and float32 ranks near -100 would tie where the sums do not.  Order: the larger rank,
 // then the lower beam, then the larger logit, then the lower token.
+//
+// The n best are found top down.  A node (a tile of a row, a chunk of a tile, 16 bytes of a chunk) is
+// worth its largest logit's continuation; the n best nodes of a level, in the order above with a
+// node's first token for its token, hold the n best continuations.  So a level is one selection: from
+// all tiles, from the chunks of about n tiles, from the logits of about n chunks.
 #pragma once
 #include "beam_tiles.cuh"
 
 namespace leat {
 
 constexpr int BM_MAX_BEAMS = 64;
-constexpr int BM_SHORT = 512;  // continuations that reach the bound and are then ordered
+constexpr int BM_MAX_WIDTH = 64;
+constexpr int BM_LIST = 256;    // nodes a level hands to the next
+constexpr int BM_PARTS = 128;   // parts of the block whose best bound a level: at least twice the width
 
 struct MergeParams {
   TileParams T;
@@ -28,7 +35,7 @@ struct MergeParams {
 
 struct LogprobParams {
   TileParams T;
-  int fmt, given, top;
+  int given, top;
   const int32_t* ids;  // (rows, given) or NULL
   float* out_given;    // (rows, given)
   float* out_top;      // (rows, top)
@@ -42,195 +49,388 @@ struct LogSum {
   float max;  // -inf: the row has no logit above -inf
   double log;
 };
-__device__ __forceinline__ LogSum row_log_sum(const TileHead* heads, int tiles, int lane) {
-  float m = neg_inf();
-  for (int t = lane; t < tiles; t += 32) m = fmaxf(m, heads[t].max);
+// (where a tile or the row's maximum is beyond PLAIN_LIMIT: kept out of line, since it hardly ever runs)
+__device__ __noinline__ double part_beyond(TileHead v, float m, int e) {
+  const double log2e_used = (double)log2e();
+  if (!(v.max > neg_inf())) return 0.0;
+  if (e != OVER_MAX) return v.sum * exp2((double)v.max * log2e_used - (double)e);
+  return v.sum * (v.exponent != OVER_MAX ? exp2((double)v.exponent - (double)m * log2e_used) : exp((double)v.max - (double)m));
+}
+// h: the lane's header of the first 32 (whatever it reads where lane >= tiles)
+__device__ __forceinline__ LogSum row_log_sum(TileHead h, const TileHead* heads, int tiles, int lane) {
+  // float32 log2e is off by a part in 2^26: the sums are of e^(x (1 + off)), which the first-order
+  // term off * max takes back but for off * (max - x), 2e-7 at most where x counts
+  const double ln2_exact = 0.693147180559945309, off = 1.44269502162933349609375 * ln2_exact - 1.0;
+  float m = lane < tiles ? h.max : neg_inf();
+  for (int t = lane + 32; t < tiles; t += 32) m = fmaxf(m, heads[t].max);
   m = unord32(__reduce_max_sync(FULL, ord32(m + 0.0f)));
-  double s = 0.0;
-  if (m > neg_inf())
-    for (int t = lane; t < tiles; t += 32) {
-      const TileHead h = heads[t];
-      if (h.max > neg_inf()) s += h.sum * exp((double)h.max - (double)m);
-    }
+  if (m == neg_inf()) return LogSum{m, 0.0};
+  const bool plain = fabsf(m) < PLAIN_LIMIT;
+  const int e = plain ? (int)ceilf(m * log2e()) : OVER_MAX;
+  auto part = [&](const TileHead& v) {
+    if (!plain || (v.exponent == OVER_MAX && v.max > neg_inf())) return part_beyond(v, m, e);
+    const int d = v.exponent - e;
+    return d > -1000 && v.max > neg_inf() ? v.sum * __hiloint2double((1023 + d) << 20, 0) : 0.0;
+  };
+  double s = lane < tiles ? part(h) : 0.0;
+  for (int t = lane + 32; t < tiles; t += 32) s += part(heads[t]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(FULL, s, d);
-  return LogSum{m, m > neg_inf() ? log(s) : 0.0};
+  return LogSum{m, plain ? log(s) + ((double)e * ln2_exact - (double)m) - off * (double)m : log(s)};
 }
 
-struct Continuation {
+template <int FMT>
+__device__ __forceinline__ float one_logit(const void* logits, size_t at) {
+  if (FMT == 0) return static_cast<const float*>(logits)[at];
+  if (FMT == 1) return __bfloat162float(static_cast<const __nv_bfloat16*>(logits)[at]);
+  return __half2float(static_cast<const __half*>(logits)[at]);
+}
+
+// A row's beam: what turns its logits into ranks
+struct Beam {
+  double base;     // score of its likeliest continuation, or of the finished beam
+  double divisor;  // the length penalty of its continuations
+  float max;       // its largest logit
+  float near_base, near_scale;  // base and 1 / divisor, rounded
+  int state;       // 0 dead, 1 live, 2 finished
+};
+// +inf counts as the largest float
+__device__ __forceinline__ double score_of(const Beam& b, float x) {
+  return b.base + ((double)fminf(x, largest_float()) - (double)b.max);
+}
+// A rank to within 2^-22 of itself and of the beam's base, enough to leave most logits out: 2 to the
+// -24th for each of the base's, the scale's and the difference's rounding and for the sum's and the
+// product's.  As ordered bits, never 0; 0 for no logit, or a NaN.
+__device__ __forceinline__ unsigned near_rank(const Beam& b, float x) {
+  return x > neg_inf() ? ord32((b.near_base + (x - b.max)) * b.near_scale + 0.0f) : 0u;
+}
+
+struct Pick {  // a node, or a logit
+  float x;
+  int token, beam;  // its (first) token; beam -1: none
+};
+struct Node {
   double rank;
   unsigned long long key;  // make_key(logit, token)
   int beam;
 };
-__device__ __forceinline__ bool goes_before(const Continuation& a, const Continuation& b) {
+__device__ __forceinline__ Node node_of(const Beam* beams, const Pick& p) {
+  const Beam& b = beams[p.beam];
+  const double score = score_of(b, p.x);
+  return Node{b.divisor == 1.0 ? score : score / b.divisor, make_key(p.x, (uint32_t)p.token), p.beam};
+}
+__device__ __forceinline__ bool goes_before(const Node& a, const Node& b) {
   if (a.rank != b.rank) return a.rank > b.rank;
   if (a.beam != b.beam) return a.beam < b.beam;
   return a.key > b.key;
 }
-// a key's logit less its row's maximum; +inf counts as the largest float
-__device__ __forceinline__ double below_max(unsigned long long key, float max) {
-  return (double)fminf(key_value(key), largest_float()) - (double)max;
+
+template <int THREADS>
+struct Level {
+  Beam beams[BM_MAX_BEAMS];
+  float reach;  // largest |near_base * near_scale| of the beams
+  Pick list[2][BM_LIST];
+  unsigned part_best[BM_PARTS];
+  int found[2];  // (one per list: a slow thread may still read one while the next level clears the other)
+  Node warp_best[THREADS / 32];
+  Pick warp_pick[THREADS / 32];
+};
+
+// The `want` best nodes, one after the other: what best_nodes comes to where its list would overflow
+template <int THREADS, typename Each>
+__device__ __noinline__ void one_by_one(Level<THREADS>& L, int which, int n, int want, Each each) {
+  constexpr int WARPS = THREADS / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  Node last{0.0, 0ull, -1};
+#pragma unroll 1
+  for (int r = 0; r < want; ++r) {
+    Node mine{0.0, 0ull, -1};
+#pragma unroll 1
+    for (int i = tid; i < n; i += THREADS)
+      each(i, [&](float x, int k, int token) {
+        if (!(x > neg_inf())) return;
+        const Node v = node_of(L.beams, Pick{x, token, k});
+        if ((last.beam < 0 || goes_before(last, v)) && (mine.beam < 0 || goes_before(v, mine))) mine = v;
+      });
+    __syncwarp();
+#pragma unroll 1
+    for (int d = 16; d > 0; d >>= 1) {
+      Node o;
+      o.rank = __shfl_xor_sync(FULL, mine.rank, d);
+      o.key = __shfl_xor_sync(FULL, mine.key, d);
+      o.beam = __shfl_xor_sync(FULL, mine.beam, d);
+      if (o.beam >= 0 && (mine.beam < 0 || goes_before(o, mine))) mine = o;
+    }
+    if (lane == 0) L.warp_best[warp] = mine;
+    __syncthreads();
+    mine = L.warp_best[0];
+#pragma unroll 1
+    for (int w = 1; w < WARPS; ++w) {
+      const Node o = L.warp_best[w];
+      if (o.beam >= 0 && (mine.beam < 0 || goes_before(o, mine))) mine = o;
+    }
+    last = mine;  // (there is one: more than `want` were found)
+    if (tid == 0) L.list[which][r] = Pick{key_value(last.key), key_id(last.key), last.beam};
+    __syncthreads();
+  }
 }
 
-// one block per group
-template <int THREADS>
-__global__ void __launch_bounds__(THREADS) beam_merge_kernel(const MergeParams P) {
-  constexpr int WARPS = THREADS / 32, AHEAD = 4;
-  __shared__ double base[BM_MAX_BEAMS];     // score of the likeliest continuation, or of a finished beam
-  __shared__ float row_max[BM_MAX_BEAMS];
-  __shared__ double divisor[BM_MAX_BEAMS];  // the length penalty of its continuations
-  __shared__ signed char state[BM_MAX_BEAMS];  // 0 dead, 1 live, 2 finished
-  __shared__ unsigned thread_best[THREADS];
-  __shared__ Continuation chosen[BM_SHORT];
-  __shared__ Continuation warp_best[WARPS];
-  __shared__ unsigned bound_bits;
-  __shared__ int found;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int group = blockIdx.x, row0 = group * P.beams, tiles = P.T.tiles;
-  const TileHead* heads = P.T.heads + (size_t)row0 * tiles;
-  const unsigned long long* lists = P.T.lists + (size_t)row0 * tiles * P.T.places;
-  grid_dependency_wait();
-  grid_launch_dependents();
-  if (tid == 0) found = 0;
-  for (int k = warp; k < P.beams; k += WARPS) {
-    const float score = P.T.scores[row0 + k];
-    const bool finished = P.T.finished && P.T.finished[row0 + k];
-    const bool live = row_is_live(P.T.scores, P.T.finished, row0 + k);
-    LogSum sum = {0.0f, 0.0};
-    if (live) sum = row_log_sum(heads + (size_t)k * tiles, tiles, lane);
-    if (lane == 0) {
-      base[k] = (double)score - sum.log;
-      row_max[k] = sum.max;
-      state[k] = live ? 1 : (finished && fabsf(score) <= largest_float() ? 2 : 0);
-      divisor[k] = P.length_penalty == 0.0f ? 1.0
-                   : pow((5.0 + (double)(P.lengths[row0 + k] + (finished ? 0 : 1))) / 6.0, (double)P.length_penalty);
-    }
-  }
-  __syncthreads();
-
-  const int segments = P.beams * tiles;
-  auto live_one = [&](int k, unsigned long long key) {
-    return Continuation{(base[k] + below_max(key, row_max[k])) / divisor[k], key, k};
-  };
-  // every continuation of the group, a warp per tile's list
-  auto each = [&](auto&& visit) {
-    for (int k = tid; k < P.beams; k += THREADS)
-      if (state[k] == 2) visit(Continuation{base[k] / divisor[k], make_key(0.0f, (uint32_t)P.end_id), k});
-#pragma unroll 1
-    for (int first = warp; first < segments; first += WARPS * AHEAD) {
-      int n[AHEAD], beam[AHEAD];
-      unsigned long long key[AHEAD];
-#pragma unroll
-      for (int a = 0; a < AHEAD; ++a) {
-        const int seg = first + a * WARPS;
-        beam[a] = seg < segments ? seg / tiles : 0;
-        n[a] = seg < segments && state[beam[a]] == 1 ? heads[seg].n : 0;
-      }
-#pragma unroll
-      for (int a = 0; a < AHEAD; ++a)
-        if (lane < n[a]) key[a] = lists[(size_t)(first + a * WARPS) * P.T.places + lane];
-#pragma unroll
-      for (int a = 0; a < AHEAD; ++a) {
-        if (lane < n[a]) visit(live_one(beam[a], key[a]));
-        for (int i = lane + 32; i < n[a]; i += 32) {
-          const unsigned long long more = lists[(size_t)(first + a * WARPS) * P.T.places + i];
-          visit(live_one(beam[a], more));
-        }
-      }
-    }
-  };
-
-  // a rank that at least `width` continuations reach: the width-th best of the threads' best
-  // (rounded down to float32, so that nothing at or above it is missed)
+// The `want` best of n nodes, and possibly a few more, into L.list[which], in no order; returns how
+// many.  Every part of the block takes its best near rank, and each warp finds, by bisection, a bound
+// that at least `want` of the parts reach; what is not clearly below it goes on the list.  If that is
+// more than the list holds (equal ranks, most of all), the nodes are taken one after the other.
+//   peek(i, beam): node i's largest logit, and its beam
+//   each(i, visit): calls visit(logit, beam, first token) for what node i puts on the list: itself,
+//                   or, at the last level, its logits
+template <int THREADS, typename Peek, typename Each>
+__device__ __forceinline__ int best_nodes(Level<THREADS>& L, int which, int n, int want, Peek peek, Each each) {
+  constexpr int LANES = THREADS / BM_PARTS, AHEAD = 4, PER_LANE = BM_PARTS / 32;
+  const int tid = threadIdx.x, lane = tid & 31;
+  unsigned first[AHEAD];  // of the thread's first nodes: usually all it has
   unsigned best = 0u;
-  each([&](const Continuation& c) { best = max(best, ord32(__double2float_rd(c.rank) + 0.0f)); });
-  thread_best[tid] = best;
-  __syncthreads();
-  if (warp == 0) {
-    unsigned v[WARPS], hi = 0u;
+  auto look = [&](int base, unsigned (&bits)[AHEAD]) {
+    float x[AHEAD];
+    int beam[AHEAD];
 #pragma unroll
-    for (int j = 0; j < WARPS; ++j) {
-      v[j] = thread_best[j * 32 + lane];
-      hi = max(hi, v[j]);
+    for (int a = 0; a < AHEAD; ++a) {
+      const int i = base + a * THREADS + tid;
+      x[a] = neg_inf();
+      beam[a] = 0;
+      if (i < n) x[a] = peek(i, beam[a]);
     }
-    unsigned lo = 0u;  // (0: threads without any; everything is taken)
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) bits[a] = near_rank(L.beams[beam[a]], x[a]);
+  };
+  look(0, first);
+#pragma unroll
+  for (int a = 0; a < AHEAD; ++a) best = max(best, first[a]);
+#pragma unroll 1
+  for (int base = THREADS * AHEAD; base < n; base += THREADS * AHEAD) {
+    unsigned bits[AHEAD];
+    look(base, bits);
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) best = max(best, bits[a]);
+  }
+#pragma unroll
+  for (int d = 1; d < LANES; d *= 2) best = max(best, __shfl_xor_sync(FULL, best, d));
+  if (tid % LANES == 0) L.part_best[tid / LANES] = best;
+  if (tid == 0) L.found[which] = 0;
+  __syncthreads();
+  unsigned bound;
+  {
+    unsigned v[PER_LANE], hi = 0u, lo = 0xFFFFFFFFu;
+#pragma unroll
+    for (int j = 0; j < PER_LANE; ++j) {
+      v[j] = L.part_best[j * 32 + lane];
+      hi = max(hi, v[j]);
+      lo = min(lo, v[j]);
+    }
+    lo = __reduce_min_sync(FULL, want <= 32 ? hi : lo);  // (each lane has one at least as large as its largest)
     hi = __reduce_max_sync(FULL, hi) + 1u;
+    const int enough = want + want / 2 + 4;
 #pragma unroll 1
     while (hi - lo > 1u) {
       const unsigned mid = lo + (hi - lo) / 2u;
       int c = 0;
 #pragma unroll
-      for (int j = 0; j < WARPS; ++j) c += v[j] >= mid ? 1 : 0;
+      for (int j = 0; j < PER_LANE; ++j) c += v[j] >= mid ? 1 : 0;
       c = __reduce_add_sync(FULL, c);
-      if (c >= P.width) lo = mid; else hi = mid;
-      if (c == P.width) break;
+      if (c >= want) lo = mid; else hi = mid;
+      if (c >= want && c <= enough) break;
     }
-    if (lane == 0) bound_bits = lo;
+    bound = 1u;  // (0: fewer parts than wanted have any; all nodes are taken)
+    if (lo > 0u) {
+      const float b = unord32(lo);
+      if (b > neg_inf()) bound = ord32(b - 9.5367431640625e-07f * (fabsf(b) + L.reach) + 0.0f);  // 2^-20: both sides' errors
+    }
+  }
+  auto put = [&](float x, int k, int token) {
+    if (near_rank(L.beams[k], x) >= bound) {
+      const int at = atomicAdd(&L.found[which], 1);
+      if (at < BM_LIST) L.list[which][at] = Pick{x, token, k};
+    }
+  };
+#pragma unroll 1
+  for (int base = 0; base < n; base += THREADS * AHEAD) {
+    unsigned bits[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) bits[a] = first[a];
+    if (base > 0) look(base, bits);
+    unsigned hits = 0u;
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) hits |= (bits[a] >= bound ? 1u : 0u) << a;
+#pragma unroll 1
+    while (hits) {
+      const int a = __ffs(hits) - 1;
+      hits &= hits - 1u;
+      each(base + a * THREADS + tid, put);
+    }
   }
   __syncthreads();
-  const unsigned bound = bound_bits;
-  each([&](const Continuation& c) {
-    if (ord32(__double2float_rd(c.rank) + 0.0f) >= bound) {
-      const int at = atomicAdd(&found, 1);
-      if (at < BM_SHORT) chosen[at] = c;
-    }
-  });
-  __syncthreads();
-  const int all = found;
+  const int found = L.found[which];
+  if (found <= BM_LIST) return found;
+  one_by_one<THREADS>(L, which, n, want, each);
+  return want;
+}
 
-  auto write = [&](int j, const Continuation& c) {
-    const size_t at = (size_t)group * P.width + j;
+// The `want` best continuations of a group's live rows (and possibly a few more) into L.list[0];
+// returns how many.  VEC as for the tiles.
+template <int THREADS, int FMT, bool VEC>
+__device__ __forceinline__ int best_of_rows(Level<THREADS>& L, const TileParams& T, int row0, int rows, int want) {
+  constexpr int PER = FMT == 0 ? 4 : 8, CHUNK = 32 * PER, TILE = BT_CHUNKS * CHUNK;
+  const int tiles = T.tiles;
+  const TileHead* heads = T.heads + (size_t)row0 * tiles;
+  const float* chunk_max = T.chunk_max + (size_t)row0 * tiles * BT_CHUNKS;
+  auto itself = [](auto peek, auto token_of) {
+    return [=](int i, auto&& visit) {
+      int k;
+      const float x = peek(i, k);
+      visit(x, k, token_of(i, k));
+    };
+  };
+  // tiles, unless there are so few that their chunks may as well be looked at
+  int n = rows * tiles;
+  const bool narrow = n > 2 * want && n * (long long)BT_CHUNKS > 4 * THREADS;
+  if (narrow) {
+    auto peek = [=, &L](int i, int& k) {
+      k = i / tiles;
+      return L.beams[k].state == 1 ? heads[i].max : neg_inf();
+    };
+    auto token_of = [=](int i, int k) { return (i - k * tiles) * TILE; };
+    n = best_nodes<THREADS>(L, 0, n, want, peek, itself(peek, token_of));
+  }
+  {
+    auto place = [=, &L](int i, int& k) {  // chunk of the group (below 2^31: checked on the host)
+      const int t = i / BT_CHUNKS, c = i % BT_CHUNKS;
+      if (!narrow) {
+        k = t / tiles;
+        return i;
+      }
+      k = L.list[0][t].beam;
+      return (k * tiles + L.list[0][t].token / TILE) * BT_CHUNKS + c;
+    };
+    auto peek = [=, &L](int i, int& k) {
+      const int at = place(i, k);
+      return L.beams[k].state == 1 ? chunk_max[at] : neg_inf();
+    };
+    auto token_of = [=](int i, int) {
+      int k;
+      const int at = place(i, k);
+      return (at - k * tiles * BT_CHUNKS) * CHUNK;
+    };
+    n = best_nodes<THREADS>(L, 1, n * BT_CHUNKS, want, peek, itself(peek, token_of));
+  }
+  // a node is 16 bytes of a chunk; it puts its logits on the list
+  auto load = [=, &L, &T](int i, int& k, int& token, uint32_t (&w)[4]) {
+    const Pick& chunk = L.list[1][i / 32];
+    k = chunk.beam;
+    token = chunk.token + (i % 32) * PER;
+    const size_t at = (size_t)(row0 + k) * T.row_stride + token;
+    const uint32_t none = FMT == 0 ? 0xFF800000u : (FMT == 1 ? 0xFF80FF80u : 0xFC00FC00u);
+    w[0] = w[1] = w[2] = w[3] = none;
+    if (VEC) {
+      if (token < T.vocab) {
+        const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const char*>(T.logits) + at * (FMT == 0 ? 4 : 2));
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+      }
+    } else if (FMT == 0) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (token + q < T.vocab) w[q] = static_cast<const uint32_t*>(T.logits)[at + q];
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (token + q < T.vocab) {
+          const uint32_t v = static_cast<const unsigned short*>(T.logits)[at + q];
+          w[q >> 1] = (q & 1) ? (w[q >> 1] & 0xFFFFu) | (v << 16) : (w[q >> 1] & 0xFFFF0000u) | v;
+        }
+    }
+  };
+  auto peek = [=](int i, int& k) {
+    int token;
+    uint32_t w[4];
+    load(i, k, token, w);
+    return largest_of<FMT>(w[0], w[1], w[2], w[3]);
+  };
+  auto each = [=](int i, auto&& visit) {
+    int k, token;
+    uint32_t w[4];
+    load(i, k, token, w);
+#pragma unroll
+    for (int q = 0; q < PER; ++q) visit(held<FMT>(w, q), k, token + q);
+  };
+  return best_nodes<THREADS>(L, 0, n * 32, want, peek, each);
+}
+
+// the length penalty: ((5 + length) / 6)^alpha
+__device__ __noinline__ double length_divisor(int length, float alpha) {
+  return pow((5.0 + (double)max(length, 0)) / 6.0, (double)alpha);
+}
+
+// one block per group
+template <int THREADS, int FMT, bool VEC>
+__global__ void __launch_bounds__(THREADS) beam_merge_kernel(const MergeParams P) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ Level<THREADS> L;
+  __shared__ Node candidates[BM_LIST + BM_MAX_BEAMS];
+  __shared__ int finished_n;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int group = blockIdx.x, row0 = group * P.beams;
+  if (tid == 0) {
+    L.reach = 0.0f;
+    finished_n = 0;
+  }
+  __syncthreads();
+  grid_dependency_wait();
+  grid_launch_dependents();
+  for (int k = warp; k < P.beams; k += WARPS) {
+    // (a row's first headers are asked for with its score; those of a row that is not live hold nothing)
+    const TileHead* heads = P.T.heads + (size_t)(row0 + k) * P.T.tiles;
+    TileHead h = {neg_inf(), 0, 0.0};
+    if (lane < P.T.tiles) h = heads[lane];
+    const float score = P.T.scores[row0 + k];
+    const bool done = P.T.finished && P.T.finished[row0 + k];
+    const bool live = fabsf(score) <= largest_float() && !done;
+    LogSum sum = {0.0f, 0.0};
+    if (live) sum = row_log_sum(h, heads, P.T.tiles, lane);
+    if (lane == 0) {
+      Beam b;
+      b.base = (double)score - sum.log;
+      b.max = sum.max;
+      b.state = live && sum.max > neg_inf() ? 1 : (done && fabsf(score) <= largest_float() ? 2 : 0);
+      b.divisor = P.length_penalty == 0.0f ? 1.0 : length_divisor(P.lengths[row0 + k] + (done ? 0 : 1), P.length_penalty);
+      b.near_base = (float)b.base;
+      b.near_scale = (float)(1.0 / b.divisor);
+      L.beams[k] = b;
+      if (b.state == 1) atomicMax(reinterpret_cast<int*>(&L.reach), __float_as_int(fabsf(b.near_base * b.near_scale)));
+    }
+  }
+  __syncthreads();
+  const int live_n = best_of_rows<THREADS, FMT, VEC>(L, P.T, row0, P.beams, P.width);
+  for (int i = tid; i < live_n; i += THREADS) candidates[i] = node_of(L.beams, L.list[0][i]);
+  if (P.T.finished)
+    for (int k = tid; k < P.beams; k += THREADS)
+      if (L.beams[k].state == 2)
+        candidates[live_n + atomicAdd(&finished_n, 1)] = Node{L.beams[k].base / L.beams[k].divisor, make_key(0.0f, (uint32_t)P.end_id), k};
+  __syncthreads();
+  const int all = live_n + finished_n;
+  for (int i = tid; i < all; i += THREADS) {
+    const Node c = candidates[i];
+    int before = 0;
+    for (int j = 0; j < all; ++j) before += goes_before(candidates[j], c) ? 1 : 0;
+    if (before >= P.width) continue;
+    const size_t at = (size_t)group * P.width + before;
     const int token = key_id(c.key);
-    const bool was = state[c.beam] == 2;
+    const Beam& b = L.beams[c.beam];
+    const bool was = b.state == 2;
     P.out_tokens[at] = token;
     P.out_parents[at] = c.beam;
-    P.out_scores[at] = (float)(was ? base[c.beam] : base[c.beam] + below_max(c.key, row_max[c.beam]));
+    P.out_scores[at] = (float)(was ? b.base : score_of(b, key_value(c.key)));
     if (P.out_finished) P.out_finished[at] = was || token == P.end_id ? 1 : 0;
     if (P.out_lengths) P.out_lengths[at] = P.lengths[row0 + c.beam] + (was ? 0 : 1);
-  };
-  int n;
-  if (all <= BM_SHORT) {
-    n = min(all, P.width);
-    for (int i = tid; i < all; i += THREADS) {
-      const Continuation c = chosen[i];
-      int before = 0;
-      for (int j = 0; j < all; ++j) before += goes_before(chosen[j], c) ? 1 : 0;
-      if (before < P.width) write(before, c);
-    }
-  } else {
-    // too many equal ranks (or all large ones with few threads): one after the other, each the best
-    // of those after the last
-    Continuation last{0.0, 0ull, -1};
-    n = 0;
-#pragma unroll 1
-    for (; n < P.width; ++n) {
-      Continuation mine{0.0, 0ull, -1};
-      each([&](const Continuation& c) {
-        if ((last.beam < 0 || goes_before(last, c)) && (mine.beam < 0 || goes_before(c, mine))) mine = c;
-      });
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) {
-        Continuation o;
-        o.rank = __shfl_xor_sync(FULL, mine.rank, d);
-        o.key = __shfl_xor_sync(FULL, mine.key, d);
-        o.beam = __shfl_xor_sync(FULL, mine.beam, d);
-        if (o.beam >= 0 && (mine.beam < 0 || goes_before(o, mine))) mine = o;
-      }
-      __syncthreads();  // (the round before has been read)
-      if (lane == 0) warp_best[warp] = mine;
-      __syncthreads();
-      mine = warp_best[0];
-#pragma unroll 1
-      for (int w = 1; w < WARPS; ++w) {
-        const Continuation o = warp_best[w];
-        if (o.beam >= 0 && (mine.beam < 0 || goes_before(o, mine))) mine = o;
-      }
-      last = mine;  // (there is one: more than `width` were counted)
-      if (tid == 0) write(n, last);
-    }
   }
   // places without a continuation: no token, no score, the beam of the place itself as parent
-  for (int j = n + tid; j < P.width; j += THREADS) {
+  for (int j = min(all, P.width) + tid; j < P.width; j += THREADS) {
     const size_t at = (size_t)group * P.width + j;
     P.out_tokens[at] = -1;
     P.out_parents[at] = j % P.beams;
@@ -241,110 +441,44 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(const MergeParams P
 }
 
 constexpr int LP_THREADS = 128;
-constexpr int LP_SHORT = 512;
 
 // one block per row
+template <int FMT, bool VEC>
 __global__ void __launch_bounds__(LP_THREADS) logprob_kernel(const LogprobParams P) {
-  constexpr int WARPS = LP_THREADS / 32;
-  __shared__ unsigned thread_best[LP_THREADS];
-  __shared__ unsigned long long chosen[LP_SHORT];
-  __shared__ unsigned long long warp_best[WARPS];
-  __shared__ unsigned bound_bits;
-  __shared__ int found;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.x, tiles = P.T.tiles;
-  const TileHead* heads = P.T.heads + (size_t)row * tiles;
-  const unsigned long long* lists = P.T.lists + (size_t)row * tiles * P.T.places;
+  __shared__ Level<LP_THREADS> L;
+  __shared__ unsigned long long keys[BM_LIST];
+  const int tid = threadIdx.x, lane = tid & 31, row = blockIdx.x;
   grid_dependency_wait();
   grid_launch_dependents();
-  if (tid == 0) found = 0;
-  const LogSum sum = row_log_sum(heads, tiles, lane);
+  const TileHead* heads = P.T.heads + (size_t)row * P.T.tiles;
+  TileHead h = {neg_inf(), 0, 0.0};
+  if (lane < P.T.tiles) h = heads[lane];
+  const LogSum sum = row_log_sum(h, heads, P.T.tiles, lane);
+  const Beam own{-sum.log, 1.0, sum.max, (float)-sum.log, 1.0f, sum.max > neg_inf() ? 1 : 0};
   for (int g = tid; g < P.given; g += LP_THREADS) {
     const int id = P.ids[(size_t)row * P.given + g];
     float x = neg_inf();  // ids outside the vocabulary have probability zero
-    if (id >= 0 && id < P.T.vocab) {
-      const size_t at = (size_t)row * P.T.row_stride + id;
-      if (P.fmt == 0) x = static_cast<const float*>(P.T.logits)[at];
-      else if (P.fmt == 1) x = __bfloat162float(static_cast<const __nv_bfloat16*>(P.T.logits)[at]);
-      else x = __half2float(static_cast<const __half*>(P.T.logits)[at]);
-    }
-    P.out_given[(size_t)row * P.given + g] =
-        x > neg_inf() ? (float)((double)fminf(x, largest_float()) - (double)sum.max - sum.log) : neg_inf();  // (NaN as -inf)
+    if (id >= 0 && id < P.T.vocab) x = one_logit<FMT>(P.T.logits, (size_t)row * P.T.row_stride + id);
+    P.out_given[(size_t)row * P.given + g] = x > neg_inf() ? (float)score_of(own, x) : neg_inf();  // (NaN as -inf)
   }
   if (P.top == 0) return;
-
-  auto each = [&](auto&& visit) {
-#pragma unroll 1
-    for (int t = warp; t < tiles; t += WARPS) {
-      const int n = heads[t].n;
-      for (int i = lane; i < n; i += 32) visit(lists[(size_t)t * P.T.places + i]);
-    }
-  };
-  unsigned best = 0u;
-  each([&](unsigned long long key) { best = max(best, key_vbits(key)); });
-  thread_best[tid] = best;
-  __syncthreads();
-  if (warp == 0) {
-    unsigned v[WARPS], hi = 0u, lo = 0u;
-#pragma unroll
-    for (int j = 0; j < WARPS; ++j) {
-      v[j] = thread_best[j * 32 + lane];
-      hi = max(hi, v[j]);
-    }
-    hi = __reduce_max_sync(FULL, hi) + 1u;
-#pragma unroll 1
-    while (hi - lo > 1u) {
-      const unsigned mid = lo + (hi - lo) / 2u;
-      int c = 0;
-#pragma unroll
-      for (int j = 0; j < WARPS; ++j) c += v[j] >= mid ? 1 : 0;
-      c = __reduce_add_sync(FULL, c);
-      if (c >= P.top) lo = mid; else hi = mid;
-      if (c == P.top) break;
-    }
-    if (lane == 0) bound_bits = lo;
+  if (tid == 0) {
+    L.beams[0] = own;
+    L.reach = fabsf(own.near_base);
   }
   __syncthreads();
-  const unsigned bound = bound_bits;
-  each([&](unsigned long long key) {
-    if (key_vbits(key) >= bound) {
-      const int at = atomicAdd(&found, 1);
-      if (at < LP_SHORT) chosen[at] = key;
-    }
-  });
+  const int all = best_of_rows<LP_THREADS, FMT, VEC>(L, P.T, row, 1, P.top);
+  for (int i = tid; i < all; i += LP_THREADS) keys[i] = make_key(L.list[0][i].x, (uint32_t)L.list[0][i].token);
   __syncthreads();
-  const int all = found;
-  auto write = [&](int j, unsigned long long key) {
-    P.out_top[(size_t)row * P.top + j] = (float)(below_max(key, sum.max) - sum.log);
-    P.out_top_ids[(size_t)row * P.top + j] = key_id(key);
-  };
-  int n;
-  if (all <= LP_SHORT) {
-    n = min(all, P.top);
-    for (int i = tid; i < all; i += LP_THREADS) {
-      const unsigned long long key = chosen[i];
-      int before = 0;
-      for (int j = 0; j < all; ++j) before += chosen[j] > key ? 1 : 0;
-      if (before < P.top) write(before, key);
-    }
-  } else {
-    unsigned long long last = ~0ull;
-    n = 0;
-#pragma unroll 1
-    for (; n < P.top; ++n) {
-      unsigned long long mine = 0ull;
-      each([&](unsigned long long key) { if (key < last && key > mine) mine = key; });
-      mine = warp_max_u64(mine);
-      __syncthreads();
-      if (lane == 0) warp_best[warp] = mine;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) mine = warp_best[w] > mine ? warp_best[w] : mine;
-      last = mine;
-      if (tid == 0) write(n, last);
-    }
+  for (int i = tid; i < all; i += LP_THREADS) {
+    const unsigned long long key = keys[i];  // (one beam: its keys' order is the order)
+    int before = 0;
+    for (int j = 0; j < all; ++j) before += keys[j] > key ? 1 : 0;
+    if (before >= P.top) continue;
+    P.out_top[(size_t)row * P.top + before] = (float)score_of(own, key_value(key));
+    P.out_top_ids[(size_t)row * P.top + before] = key_id(key);
   }
-  for (int j = n + tid; j < P.top; j += LP_THREADS) {
+  for (int j = min(all, P.top) + tid; j < P.top; j += LP_THREADS) {
     P.out_top[(size_t)row * P.top + j] = neg_inf();
     P.out_top_ids[(size_t)row * P.top + j] = -1;
   }

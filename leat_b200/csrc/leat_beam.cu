@@ -18,21 +18,21 @@ namespace {
 
 constexpr int kMaxGroups = 65535;  // a grid's second dimension
 constexpr long long kMaxBlocks = 0x7FFFFFFF;
+constexpr int MERGE_THREADS = 256;
 
 struct Scratch {
-  int tiles, places;
-  size_t lists_at, total;
+  int tiles;
+  size_t chunks_at, total;
 };
 
-// headers, then (with candidates) the tiles' lists
-Scratch scratch_for(int rows, int vocab, int top, bool half) {
+// headers, then the maxima of the tiles' chunks where anything is to be selected
+Scratch scratch_for(int rows, int vocab, int width, bool half) {
   Scratch s;
   const int tile = tile_logits(half);
   s.tiles = (int)(((long long)vocab + tile - 1) / tile);
-  s.places = top > 0 ? top + BT_SLACK : 0;
   const size_t cells = (size_t)rows * s.tiles;
-  s.lists_at = (cells * sizeof(TileHead) + 255) / 256 * 256;
-  s.total = s.lists_at + cells * s.places * 8;
+  s.chunks_at = (cells * sizeof(TileHead) + 255) / 256 * 256;
+  s.total = s.chunks_at + (width > 0 ? cells * BT_CHUNKS * 4 : 0);
   return s;
 }
 
@@ -40,30 +40,43 @@ bool known_format(uint32_t flags) {
   return (flags & ~(uint32_t)(LEAT_FLAG_LOGITS_BF16 | LEAT_FLAG_LOGITS_F16)) == 0 &&
          flags != (uint32_t)(LEAT_FLAG_LOGITS_BF16 | LEAT_FLAG_LOGITS_F16);
 }
-int format_of(uint32_t flags) { return flags & LEAT_FLAG_LOGITS_BF16 ? 1 : (flags & LEAT_FLAG_LOGITS_F16 ? 2 : 0); }
-
-template <int FMT, bool VEC>
-cudaError_t launch_tiles(const TileParams& T, int rows, cudaStream_t stream) {
-  const dim3 grid((unsigned)((long long)rows * T.tiles));
-  return T.top > 0 ? launch_dependent(beam_tile_kernel<FMT, VEC, true>, grid, dim3(BT_THREADS), 0, stream, T)
-                   : launch_dependent(beam_tile_kernel<FMT, VEC, false>, grid, dim3(BT_THREADS), 0, stream, T);
-}
 
 // whole 16-byte vectors where the rows allow it, one logit per load elsewhere: the same for every row
 // of a call, so that equal rows have equal sums
-int stream_tiles(const TileParams& T, int fmt, int rows, cudaStream_t stream) {
-  const int per_vec = fmt == 0 ? 4 : 8;
+template <template <int, bool> class Launch, typename Params>
+cudaError_t by_format(const Params& P, uint32_t flags, int rows, int blocks, cudaStream_t stream) {
+  const TileParams& T = P.T;
+  const int per_vec = flags == 0 ? 4 : 8;
   const bool vec = T.vocab % per_vec == 0 && T.row_stride % per_vec == 0 && aligned(T.logits, 16);
-  cudaError_t e;
-  if (fmt == 0) e = vec ? launch_tiles<0, true>(T, rows, stream) : launch_tiles<0, false>(T, rows, stream);
-  else if (fmt == 1) e = vec ? launch_tiles<1, true>(T, rows, stream) : launch_tiles<1, false>(T, rows, stream);
-  else e = vec ? launch_tiles<2, true>(T, rows, stream) : launch_tiles<2, false>(T, rows, stream);
-  return cuda_failed(e, "beam_tile_kernel launch") ? LEAT_E_CUDA : LEAT_OK;
+  if (flags == 0) return vec ? Launch<0, true>::both(P, rows, blocks, stream) : Launch<0, false>::both(P, rows, blocks, stream);
+  if (flags & LEAT_FLAG_LOGITS_BF16) return vec ? Launch<1, true>::both(P, rows, blocks, stream) : Launch<1, false>::both(P, rows, blocks, stream);
+  return vec ? Launch<2, true>::both(P, rows, blocks, stream) : Launch<2, false>::both(P, rows, blocks, stream);
 }
+
+template <int FMT, bool VEC>
+struct Tiles {
+  static cudaError_t launch(const TileParams& T, int rows, cudaStream_t stream) {
+    return launch_dependent(beam_tile_kernel<FMT, VEC>, dim3((unsigned)((long long)rows * T.tiles)), dim3(BT_THREADS), 0, stream, T);
+  }
+};
+template <int FMT, bool VEC>
+struct Select {
+  static cudaError_t both(const MergeParams& P, int rows, int groups, cudaStream_t stream) {
+    const cudaError_t e = Tiles<FMT, VEC>::launch(P.T, rows, stream);
+    return e != cudaSuccess ? e : launch_dependent(beam_merge_kernel<MERGE_THREADS, FMT, VEC>, dim3(groups), dim3(MERGE_THREADS), 0, stream, P);
+  }
+};
+template <int FMT, bool VEC>
+struct Logprobs {
+  static cudaError_t both(const LogprobParams& P, int rows, int, cudaStream_t stream) {
+    const cudaError_t e = Tiles<FMT, VEC>::launch(P.T, rows, stream);
+    return e != cudaSuccess ? e : launch_dependent(logprob_kernel<FMT, VEC>, dim3(rows), dim3(LP_THREADS), 0, stream, P);
+  }
+};
 
 bool logits_fit(const void* logits, int rows, int vocab, long long row_stride, uint32_t flags, const Scratch& s) {
   return logits && aligned(logits, flags ? 2 : 4) && (rows == 1 || row_stride >= vocab) &&
-         (long long)rows * s.tiles <= kMaxBlocks;
+         (long long)rows * s.tiles <= kMaxBlocks / BT_CHUNKS;  // (chunks are counted in 32 bits)
 }
 
 int64_t lowest_bit(int64_t x) { return x & -x; }
@@ -73,7 +86,7 @@ int64_t lowest_bit(int64_t x) { return x & -x; }
 extern "C" {
 
 size_t leat_beam_workspace_bytes(int32_t rows, int32_t vocab, int32_t width) {
-  if (rows <= 0 || vocab <= 0 || width < 0 || width > BT_MAX_TOP) return 0;
+  if (rows <= 0 || vocab <= 0 || width < 0 || width > BM_MAX_WIDTH) return 0;
   // (the smaller tiles are those of float32: enough for every format)
   return scratch_for(rows, vocab, width, false).total;
 }
@@ -82,13 +95,13 @@ int leat_beam_select(const leat_beam_args* a, leat_stream_t stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (!a) return LEAT_E_ARGUMENT;
   if (a->groups < 0 || a->beams <= 0 || a->vocab <= 0 || a->width <= 0 || !known_format(a->flags)) return LEAT_E_ARGUMENT;
-  if (a->beams > BM_MAX_BEAMS || a->width > BT_MAX_TOP) return LEAT_E_CAPACITY;
+  if (a->beams > BM_MAX_BEAMS || a->width > BM_MAX_WIDTH) return LEAT_E_CAPACITY;
   if (a->groups == 0) return LEAT_OK;
   if ((long long)a->groups * a->beams > kMaxBlocks) return LEAT_E_CAPACITY;
   const int rows = a->groups * a->beams;
   if (!a->scores || !a->out_tokens || !a->out_parents || !a->out_scores) return LEAT_E_ARGUMENT;
   if (a->end_id >= a->vocab || (a->end_id < 0 && (a->finished || a->out_finished))) return LEAT_E_ARGUMENT;
-  if (!(fabsf(a->length_penalty) <= 16.0f)) return LEAT_E_ARGUMENT;
+  if (!(fabsf(a->length_penalty) <= 4.0f)) return LEAT_E_ARGUMENT;
   if (!a->lengths && (a->length_penalty != 0.0f || a->out_lengths)) return LEAT_E_ARGUMENT;
   const Scratch s = scratch_for(rows, a->vocab, a->width, a->flags != 0);
   if (!logits_fit(a->logits, rows, a->vocab, a->row_stride, a->flags, s)) return LEAT_E_ARGUMENT;
@@ -96,25 +109,22 @@ int leat_beam_select(const leat_beam_args* a, leat_stream_t stream_) {
   MergeParams P;
   memset(&P, 0, sizeof(P));
   P.T.logits = a->logits; P.T.row_stride = a->row_stride; P.T.vocab = a->vocab;
-  P.T.tiles = s.tiles; P.T.top = a->width; P.T.places = s.places;
+  P.T.tiles = s.tiles; P.T.with_chunks = 1;
   P.T.scores = a->scores; P.T.finished = a->finished;
   P.T.heads = static_cast<TileHead*>(a->workspace);
-  P.T.lists = reinterpret_cast<unsigned long long*>(static_cast<char*>(a->workspace) + s.lists_at);
+  P.T.chunk_max = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + s.chunks_at);
   P.beams = a->beams; P.width = a->width; P.end_id = a->end_id < 0 ? -1 : a->end_id;
   P.length_penalty = a->length_penalty; P.lengths = a->lengths;
   P.out_tokens = a->out_tokens; P.out_parents = a->out_parents; P.out_scores = a->out_scores;
   P.out_finished = a->out_finished; P.out_lengths = a->out_lengths;
-  const int code = stream_tiles(P.T, format_of(a->flags), rows, stream);
-  if (code != LEAT_OK) return code;
-  return cuda_failed(launch_dependent(beam_merge_kernel<512>, dim3(a->groups), dim3(512), 0, stream, P),
-                     "beam_merge_kernel launch") ? LEAT_E_CUDA : LEAT_OK;
+  return cuda_failed(by_format<Select>(P, a->flags, rows, a->groups, stream), "beam selection launch") ? LEAT_E_CUDA : LEAT_OK;
 }
 
 int leat_token_logprobs(const leat_logprob_args* a, leat_stream_t stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (!a) return LEAT_E_ARGUMENT;
   if (a->rows < 0 || a->vocab <= 0 || a->given < 0 || a->top < 0 || !known_format(a->flags)) return LEAT_E_ARGUMENT;
-  if (a->top > BT_MAX_TOP) return LEAT_E_CAPACITY;
+  if (a->top > BM_MAX_WIDTH) return LEAT_E_CAPACITY;
   if (a->rows == 0) return LEAT_OK;
   if ((a->given > 0 && (!a->ids || !a->out_logprobs)) || (a->top > 0 && (!a->out_top_logprobs || !a->out_top_ids)))
     return LEAT_E_ARGUMENT;
@@ -124,15 +134,12 @@ int leat_token_logprobs(const leat_logprob_args* a, leat_stream_t stream_) {
   LogprobParams P;
   memset(&P, 0, sizeof(P));
   P.T.logits = a->logits; P.T.row_stride = a->row_stride; P.T.vocab = a->vocab;
-  P.T.tiles = s.tiles; P.T.top = a->top; P.T.places = s.places;
+  P.T.tiles = s.tiles; P.T.with_chunks = a->top > 0;
   P.T.heads = static_cast<TileHead*>(a->workspace);
-  P.T.lists = reinterpret_cast<unsigned long long*>(static_cast<char*>(a->workspace) + s.lists_at);
-  P.fmt = format_of(a->flags); P.given = a->given; P.top = a->top; P.ids = a->ids;
+  P.T.chunk_max = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + s.chunks_at);
+  P.given = a->given; P.top = a->top; P.ids = a->ids;
   P.out_given = a->out_logprobs; P.out_top = a->out_top_logprobs; P.out_top_ids = a->out_top_ids;
-  const int code = stream_tiles(P.T, P.fmt, a->rows, stream);
-  if (code != LEAT_OK) return code;
-  return cuda_failed(launch_dependent(logprob_kernel, dim3(a->rows), dim3(LP_THREADS), 0, stream, P),
-                     "logprob_kernel launch") ? LEAT_E_CUDA : LEAT_OK;
+  return cuda_failed(by_format<Logprobs>(P, a->flags, a->rows, 0, stream), "log-probabilities launch") ? LEAT_E_CUDA : LEAT_OK;
 }
 
 int leat_reorder_states(const leat_state* states, int32_t count, const int32_t* parents, const int32_t* slots,
