@@ -138,7 +138,8 @@ def _load() -> C.CDLL:
     lib.leat_beam_workspace_bytes.restype = sz
     lib.leat_beam_workspace_bytes.argtypes = [i32, i32, i32]
     lib.leat_beam_select.argtypes = [C.POINTER(BeamArgs), p]
-    lib.leat_reorder_states.argtypes = [C.POINTER(State), i32, p, p, i32, i32, p, i32, p, i32, p]
+    lib.leat_reorder_states.argtypes = [p, i32,  # (a State array, or its bytes)
+                                          p, p, i32, i32, p, i32, p, i32, p]
     lib.leat_beam_sequences.argtypes = [p, p, i32, i32, i32, i32, p, p, p]
     lib.leat_token_logprobs.argtypes = [C.POINTER(LogprobArgs), p]
     for name in EXPORTS:

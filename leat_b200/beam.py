@@ -9,6 +9,7 @@ scratch is its own, so every part can be captured into a CUDA graph."""
 from __future__ import annotations
 
 from dataclasses import dataclass
+from struct import pack
 
 import torch
 
@@ -17,6 +18,7 @@ from leat_b200.logprobs import FORMATS, launch, rows_of_logits, scratch
 
 MAX_BEAMS = 64
 MAX_WIDTH = 64
+STATE_WORDS = "PqqqiiiI"  # struct leat_state, with the padding at its end
 
 
 @dataclass
@@ -37,8 +39,8 @@ class Sequences:
 
 
 def _whole(x, dtype, shape, device, name: str) -> torch.Tensor:
-    if not isinstance(x, torch.Tensor) or x.dtype != dtype or x.device != device or tuple(x.shape) != shape:
-        raise ValueError(f"{name} must be a {shape} {str(dtype).removeprefix('torch.')} tensor on {device}")
+    if not isinstance(x, torch.Tensor) or x.dtype != dtype or x.shape != shape or x.device != device:
+        raise ValueError(f"{name} must be a {tuple(shape)} {str(dtype).removeprefix('torch.')} tensor on {device}")
     return x if x.is_contiguous() else x.contiguous()
 
 
@@ -65,60 +67,67 @@ def beam_select(logits, scores: torch.Tensor, width: int | None = None, *, finis
     rows, vocab = logits.shape
     if not isinstance(scores, torch.Tensor) or scores.dim() != 2:
         raise ValueError("scores must be a (G, K) float32 tensor")
-    groups, beams = scores.shape
-    scores = _whole(scores, torch.float32, (groups, beams), dev, "scores")
+    shape = scores.shape
+    groups, beams = shape
+    scores = _whole(scores, torch.float32, shape, dev, "scores")
     if not 1 <= beams <= MAX_BEAMS or groups * beams != rows:
         raise ValueError(f"logits must have a row per beam of scores (G, K), K from 1 to {MAX_BEAMS}")
-    width = beams if width is None else width
-    if isinstance(width, bool) or not isinstance(width, int) or not 1 <= width <= MAX_WIDTH:
+    if width is None:
+        width = beams
+    elif type(width) is not int or not 1 <= width <= MAX_WIDTH:
         raise ValueError(f"width must be an integer from 1 to {MAX_WIDTH}")
-    if end_id is not None and (isinstance(end_id, bool) or not isinstance(end_id, int) or not 0 <= end_id < vocab):
-        raise ValueError("end_id must be a token of the vocabulary")
-    if finished is not None:
-        if end_id is None:
-            raise ValueError("finished beams continue with end_id: give one")
-        finished = _whole(finished, torch.bool, (groups, beams), dev, "finished")
+    done_at = lengths_at = ended_at = new_lengths_at = None
+    if end_id is not None:
+        if type(end_id) is not int or not 0 <= end_id < vocab:
+            raise ValueError("end_id must be a token of the vocabulary")
+        if finished is not None:
+            finished = _whole(finished, torch.bool, shape, dev, "finished")
+            done_at = finished.data_ptr()
+    elif finished is not None:
+        raise ValueError("finished beams continue with end_id: give one")
     if lengths is not None:
-        lengths = _whole(lengths, torch.int32, (groups, beams), dev, "lengths")
+        lengths = _whole(lengths, torch.int32, shape, dev, "lengths")
+        lengths_at = lengths.data_ptr()
+        if not -4.0 <= length_penalty <= 4.0:
+            raise ValueError("length_penalty must be a number from -4 to 4")
     elif length_penalty != 0.0:
         raise ValueError("length_penalty needs the beams' lengths")
-    if not -4.0 <= length_penalty <= 4.0:
-        raise ValueError("length_penalty must be a number from -4 to 4")
-    shape = (groups, width)
     if out is None:
-        tokens, parents, bits, *more = torch.empty((3 if lengths is None else 4, groups, width), dtype=torch.int32, device=dev).unbind(0)
-        out = Selected(tokens, parents, bits.view(torch.float32))
-        if lengths is not None:
-            out.lengths = more[0]
-        if end_id is not None:
-            out.finished = torch.empty(shape, dtype=torch.bool, device=dev)
+        tokens, parents, bits, *more = torch.empty(3 if lengths is None else 4, groups, width, dtype=torch.int32, device=dev).unbind(0)
+        out = Selected(tokens, parents, bits.view(torch.float32), None if end_id is None else torch.empty(groups, width, dtype=torch.bool, device=dev),
+                       None if lengths is None else more[0])  # fmt: skip
     else:
         wanted = [(out.tokens, torch.int32), (out.parents, torch.int32), (out.scores, torch.float32)]
         wanted += [(out.finished, torch.bool)] if end_id is not None else []
         wanted += [(out.lengths, torch.int32)] if lengths is not None else []
+        read = (scores.data_ptr(), lengths_at, done_at)
         for t, dtype in wanted:
-            if t is None or t.dtype != dtype or tuple(t.shape) != shape or t.device != dev or not t.is_contiguous():
-                raise ValueError(f"out must hold contiguous {shape} tensors on {dev}, of the types of a Selected")
-            if t.numel() and t.data_ptr() in (x.data_ptr() for x in (scores, finished, lengths) if x is not None):
+            if t is None or t.dtype != dtype or t.shape != (groups, width) or t.device != dev or not t.is_contiguous():
+                raise ValueError(f"out must hold contiguous ({groups}, {width}) tensors on {dev}, of the types of a Selected")
+            if t.data_ptr() in read and groups:
                 raise ValueError("out must not be what the step reads")
     if groups == 0:
         return out
+    if end_id is not None:
+        ended_at = out.finished.data_ptr()
+    if lengths is not None:
+        new_lengths_at = out.lengths.data_ptr()
     held, at, size = scratch(rows, vocab, width, dev)
     a = _lib.BeamArgs(
         logits.data_ptr(), groups, beams, vocab, width, logits.stride(0), FORMATS[logits.dtype], -1 if end_id is None else end_id,
-        scores.data_ptr(), None if finished is None else finished.data_ptr(), None if lengths is None else lengths.data_ptr(),
-        length_penalty, out.tokens.data_ptr(), out.parents.data_ptr(), out.scores.data_ptr(),
-        None if end_id is None else out.finished.data_ptr(), None if lengths is None else out.lengths.data_ptr(), at, size)  # fmt: skip
-    launch(dev, "leat_beam_select", _lib.lib.leat_beam_select, a)
+        scores.data_ptr(), done_at, lengths_at, length_penalty, out.tokens.data_ptr(), out.parents.data_ptr(), out.scores.data_ptr(),
+        ended_at, new_lengths_at, at, size)  # fmt: skip
+    launch(dev.index, "leat_beam_select", _lib.lib.leat_beam_select, a)
     return out
 
 
 def _state(t: torch.Tensor, dim: int | None) -> tuple:
-    """A tensor as leat_state has it: rows, runs of places per row, places, and their strides in bytes."""
+    """A tensor as leat_state has it behind its address: the bytes from row to row, from run to run of its
+    places and of a place, and how many runs, places and rows there are."""
     shape, stride, size = t.shape, t.stride(), t.element_size()
     if dim is None:
         if t.dim() == 1:
-            return (t.data_ptr(), stride[0] * size, 0, size, 1, 1, shape[0])
+            return (stride[0] * size, 0, size, 1, 1, shape[0])
         dim = 1
         places_are_all = True
     else:
@@ -144,7 +153,7 @@ def _state(t: torch.Tensor, dim: int | None) -> tuple:
         outer *= shape[i]
     if places_are_all:
         inner, places = inner * places, 1
-    return (t.data_ptr(), stride[0] * size, outer_stride * size, inner * size, outer, places, shape[0])
+    return (stride[0] * size, outer_stride * size, inner * size, outer, places, shape[0])
 
 
 def _overlaps(row_stride: int, outer_stride: int, place_bytes: int, outer: int, places: int, rows: int) -> bool:
@@ -198,24 +207,30 @@ def reorder_states(states, parents: torch.Tensor, *, slots: torch.Tensor | None 
         raise ValueError("start and length count positions: say which dimension they are with dim")
     start_at, start_all, keep_start = _range_end(0 if start is None else start, groups, dev, "start")
     end_at, end_all, keep_end = _range_end(0x7FFFFFFF if length is None else length, groups, dev, "length")
-    described = []
+    # a search's caches are mostly alike: what one comes to holds for the next of its shape and strides
+    words: list[int] = []
+    index, shape, stride, dtype = dev.index, None, None, None
     for t in states:
-        if not isinstance(t, torch.Tensor) or t.device != dev or t.dim() == 0 or t.layout != torch.strided or t.requires_grad:
+        if not isinstance(t, torch.Tensor) or t.get_device() != index or t.requires_grad:
             raise ValueError(f"states must be tensors on {dev}, rows first, that need no gradient")
-        if slots is None and t.shape[0] < groups * beams:
-            raise ValueError("states must have a row per beam, or slots must say which rows are the beams'")
-        if dim is not None and not 0 < dim < t.dim():
-            raise ValueError("dim must be a dimension of every state, behind the rows'")
-        if t.numel() == 0:
-            continue
-        s = _state(t, dim)
-        if _overlaps(*s[1:]):
-            raise ValueError("the rows of a state must not overlap")
-        described.append(s)
-    if not described or groups == 0:
+        if t.shape != shape or t.dtype != dtype or t.stride() != stride:
+            if t.layout is not torch.strided or t.dim() == 0:
+                raise ValueError("states must be strided tensors with their rows as first dimension")
+            if slots is None and t.shape[0] < groups * beams:
+                raise ValueError("states must have a row per beam, or slots must say which rows are the beams'")
+            if dim is not None and not 0 < dim < t.dim():
+                raise ValueError("dim must be a dimension of every state, behind the rows'")
+            if t.numel() == 0:
+                continue
+            like = _state(t, dim)
+            if _overlaps(*like):
+                raise ValueError("the rows of a state must not overlap")
+            shape, dtype, stride = t.shape, t.dtype, t.stride()
+        words += (t.data_ptr(), *like, 0)
+    if not words or groups == 0:
         return
-    array = (_lib.State * len(described))(*described)
-    launch(dev, "leat_reorder_states", _lib.lib.leat_reorder_states, array, len(described), parents.data_ptr(),
+    count = len(words) // 8
+    launch(index, "leat_reorder_states", _lib.lib.leat_reorder_states, pack(STATE_WORDS * count, *words), count, parents.data_ptr(),
            None if slots is None else slots.data_ptr(), groups, beams, start_at, start_all, end_at, end_all)  # fmt: skip
     del keep_start, keep_end
 
@@ -234,10 +249,10 @@ def beam_sequences(tokens: torch.Tensor, parents: torch.Tensor, end_id: int | No
         raise ValueError(f"there must be 1 to {MAX_BEAMS} beams")
     if end_id is not None and (isinstance(end_id, bool) or not isinstance(end_id, int) or not 0 <= end_id <= 0x7FFFFFFF):
         raise ValueError("end_id must be a token")
-    out = Sequences(torch.empty((groups, beams, steps), dtype=torch.int32, device=dev),
-                    torch.empty((groups, beams), dtype=torch.int32, device=dev))  # fmt: skip
+    out = Sequences(torch.empty(groups, beams, steps, dtype=torch.int32, device=dev),
+                    torch.empty(groups, beams, dtype=torch.int32, device=dev))  # fmt: skip
     if groups:
-        launch(dev, "leat_beam_sequences", _lib.lib.leat_beam_sequences, tokens.data_ptr(), parents.data_ptr(), steps, groups, beams,
+        launch(dev.index, "leat_beam_sequences", _lib.lib.leat_beam_sequences, tokens.data_ptr(), parents.data_ptr(), steps, groups, beams,
                -1 if end_id is None else end_id, out.tokens.data_ptr(), out.lengths.data_ptr())  # fmt: skip
     return out
 

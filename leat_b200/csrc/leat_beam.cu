@@ -211,19 +211,23 @@ int leat_beam_sequences(const int32_t* tokens, const int32_t* parents, int32_t s
   SequenceParams P;
   P.tokens = tokens; P.parents = parents; P.steps = steps; P.groups = groups; P.beams = beams;
   P.has_end = end_id >= 0; P.end_id = end_id; P.out = out_tokens; P.out_lengths = out_lengths;
-  // a cluster per group: as many blocks as leave each at least 64 steps, while the GPU has room
+  // a cluster per group: as many blocks as leave each at least 64 steps, while two fit on every SM
   int blocks = 1;
-  while (blocks < 8 && steps > 64 * blocks && (long long)groups * blocks < 2 * 148) blocks *= 2;
+  while (blocks < SQ_MAX_BLOCKS && steps > 64 * blocks && (long long)groups * blocks <= 148) blocks *= 2;
   if ((long long)groups * blocks > kMaxBlocks) return LEAT_E_CAPACITY;
   int chunk = (steps + blocks - 1) / blocks;
-  const int most = SQ_SHARED / (2 * beams);
+  const int most = SQ_SHARED / (9 * beams);
   if (chunk > most) chunk = most;
   if (chunk < 1) chunk = 1;
-  // runs: their number costs as much to compose as half their length costs to walk (twice)
-  int runs = 1;
-  while (runs * 2 * beams <= SQ_THREADS && runs * runs < 2 * chunk) runs *= 2;
-  P.chunk = chunk; P.runs = runs;
-  const size_t shared = (size_t)2 * chunk * beams;
+  chunk = (chunk + 3) / 4 * 4;  // (tokens behind the parents stay 16-byte aligned)
+  P.chunk = chunk;
+  // runs of an odd number of steps: walked side by side, they lie in different banks
+  P.run_len = (chunk + SQ_THREADS / beams - 1) / (SQ_THREADS / beams) | 1;
+  P.runs = (chunk + P.run_len - 1) / P.run_len;
+  P.vec = beams % 4 == 0 && aligned(tokens, 16) && aligned(parents, 16) ? 4 : 1;
+  const unsigned per_step = (unsigned)(beams / P.vec);
+  P.divide = (unsigned)((0x100000000ull + per_step - 1) / per_step);
+  const size_t shared = (size_t)9 * chunk * beams;
   if (shared > 40 * 1024 &&
       cuda_failed(cudaFuncSetAttribute(sequences_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared), "cudaFuncSetAttribute"))
     return LEAT_E_CUDA;

@@ -5,6 +5,7 @@ no handle, no host synchronisation; scratch is allocated per call on the current
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -24,32 +25,48 @@ class TokenLogprobs:
 
 def rows_of_logits(logits) -> torch.Tensor:
     """`logits` as the kernels take it: (B, V) on the device, adjacent logits adjacent in memory."""
-    logits = device_tensor(logits)
+    if not isinstance(logits, torch.Tensor):
+        logits = device_tensor(logits)
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in FORMATS or not logits.is_cuda:
         raise ValueError("logits must be a (B, V) float32, bfloat16 or float16 CUDA tensor")
-    if logits.shape[1] == 0:
+    rows, vocab = logits.shape
+    if vocab == 0:
         raise ValueError("logits must have at least one token per row")
-    if (logits.stride(1) != 1 and logits.shape[1] > 1) or (logits.stride(0) < logits.shape[1] and logits.shape[0] > 1):
-        logits = logits.contiguous()
+    if not logits.is_contiguous():
+        stride = logits.stride()
+        if (stride[1] != 1 and vocab > 1) or (stride[0] < vocab and rows > 1):
+            logits = logits.contiguous()
     return logits
+
+
+@lru_cache(maxsize=256)
+def _scratch_bytes(rows: int, vocab: int, width: int) -> int:
+    size = _lib.lib.leat_beam_workspace_bytes(rows, vocab, width)
+    if size == 0:
+        raise ValueError(f"({rows}, {vocab}) logits are beyond the kernels' sizes")
+    return size
 
 
 def scratch(rows: int, vocab: int, width: int, device) -> tuple[torch.Tensor, int, int]:
     """A call's workspace: the tensor that holds it, its 256-byte aligned address and its size.  It is
     the call's own (the caching allocator keeps it for the current stream), so calls on several
     streams or in several graphs share nothing."""
-    size = _lib.lib.leat_beam_workspace_bytes(rows, vocab, width)
+    size = _scratch_bytes(rows, vocab, width)
     held = torch.empty(size + 256, dtype=torch.uint8, device=device)
     return held, (held.data_ptr() + 255) & ~255, size
 
 
-def launch(device: torch.device, what: str, call, *args) -> None:
-    """call(*args, stream) on `device` and its current stream."""
-    if torch.cuda.current_device() == device.index:
-        code = call(*args, torch.cuda.current_stream().cuda_stream)
+# the current stream's handle without a Stream object around it (3 us of a 15 us call), where torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def launch(index: int, what: str, call, *args) -> None:
+    """call(*args, stream) on CUDA device `index` and its current stream."""
+    if torch.cuda.current_device() == index:
+        code = call(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            code = call(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            code = call(*args, _raw_stream(index))
     if code != _lib.OK:
         _lib.check(code, what)
 
@@ -69,18 +86,19 @@ def token_logprobs(logits, ids=None, top: int = 0) -> TokenLogprobs:
     given = 0
     if ids is not None:
         ids = device_tensor(ids)
-        if ids.dtype not in (torch.int32, torch.int64) or ids.device != dev:
+        if not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int32, torch.int64) or ids.device != dev:
             raise ValueError("ids must be an int32 or int64 tensor on the logits' device")
         if ids.dim() not in (1, 2) or ids.shape[0] != rows:
             raise ValueError("ids must be (B,) or (B, M), a row per row of logits")
+        given = ids.shape[1] if ids.dim() == 2 else 1
         if ids.dtype == torch.int64:  # (what does not fit 32 bits is outside every vocabulary)
             ids = ids.clamp(-1, vocab).to(torch.int32)
-        ids = ids.reshape(rows, -1 if rows else (ids.shape[1] if ids.dim() == 2 else 1)).contiguous()
-        given = ids.shape[1]
-    out = TokenLogprobs(torch.empty((rows, given), dtype=torch.float32, device=dev) if ids is not None else None)
+        if not ids.is_contiguous():
+            ids = ids.contiguous()
+    out = TokenLogprobs(torch.empty(rows, given, dtype=torch.float32, device=dev) if ids is not None else None)
     if top:
-        out.top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=dev)
-        out.top_ids = torch.empty((rows, top), dtype=torch.int32, device=dev)
+        out.top_logprobs = torch.empty(rows, top, dtype=torch.float32, device=dev)
+        out.top_ids = torch.empty(rows, top, dtype=torch.int32, device=dev)
     if rows == 0 or given + top == 0:
         return out
     held, at, size = scratch(rows, vocab, top, dev)
@@ -88,5 +106,5 @@ def token_logprobs(logits, ids=None, top: int = 0) -> TokenLogprobs:
         logits.data_ptr(), rows, vocab, logits.stride(0), FORMATS[logits.dtype], given, top, ids.data_ptr() if given else None,
         out.logprobs.data_ptr() if given else None, out.top_logprobs.data_ptr() if top else None,
         out.top_ids.data_ptr() if top else None, at, size)  # fmt: skip
-    launch(dev, "leat_token_logprobs", _lib.lib.leat_token_logprobs, a)
+    launch(dev.index, "leat_token_logprobs", _lib.lib.leat_token_logprobs, a)
     return out
