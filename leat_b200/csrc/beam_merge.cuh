@@ -69,8 +69,7 @@ __device__ __forceinline__ LogSum row_log_sum(TileHead h, const TileHead* heads,
   const int e = plain ? (int)ceilf(m * log2e()) : OVER_MAX;
   auto part = [&](const TileHead& v) {
     if (!plain || (v.exponent == OVER_MAX && v.max > neg_inf())) return part_beyond(v, m, e);
-    const int d = v.exponent - e;
-    return d > -1000 && v.max > neg_inf() ? v.sum * __hiloint2double((1023 + d) << 20, 0) : 0.0;
+    return v.max > neg_inf() ? v.sum * two_to(v.exponent - e) : 0.0;
   };
   double s = lane < tiles ? part(h) : 0.0;
   for (int t = lane + 32; t < tiles; t += 32) s += part(heads[t]);

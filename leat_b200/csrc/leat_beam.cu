@@ -56,7 +56,10 @@ cudaError_t by_format(const Params& P, uint32_t flags, int rows, int blocks, cud
 template <int FMT, bool VEC>
 struct Tiles {
   static cudaError_t launch(const TileParams& T, int rows, cudaStream_t stream) {
-    return launch_dependent(beam_tile_kernel<FMT, VEC>, dim3((unsigned)((long long)rows * T.tiles)), dim3(BT_THREADS), 0, stream, T);
+    // a row's tiles next to each other (the other way round, rows first, reads float32 at 5.9 TB/s for 6.7)
+    const int high = rows < kMaxGroups ? rows : 32768;
+    return launch_dependent(beam_tile_kernel<FMT, VEC>, dim3((unsigned)T.tiles, (unsigned)high, (unsigned)((rows + high - 1) / high)),
+                            dim3(BT_THREADS), 0, stream, T);
   }
 };
 template <int FMT, bool VEC>
@@ -108,7 +111,7 @@ int leat_beam_select(const leat_beam_args* a, leat_stream_t stream_) {
   if (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < s.total) return LEAT_E_WORKSPACE;
   MergeParams P;
   memset(&P, 0, sizeof(P));
-  P.T.logits = a->logits; P.T.row_stride = a->row_stride; P.T.vocab = a->vocab;
+  P.T.logits = a->logits; P.T.row_stride = a->row_stride; P.T.rows = rows; P.T.vocab = a->vocab;
   P.T.tiles = s.tiles; P.T.with_chunks = 1;
   P.T.scores = a->scores; P.T.finished = a->finished;
   P.T.heads = static_cast<TileHead*>(a->workspace);
@@ -133,7 +136,7 @@ int leat_token_logprobs(const leat_logprob_args* a, leat_stream_t stream_) {
   if (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < s.total) return LEAT_E_WORKSPACE;
   LogprobParams P;
   memset(&P, 0, sizeof(P));
-  P.T.logits = a->logits; P.T.row_stride = a->row_stride; P.T.vocab = a->vocab;
+  P.T.logits = a->logits; P.T.row_stride = a->row_stride; P.T.rows = a->rows; P.T.vocab = a->vocab;
   P.T.tiles = s.tiles; P.T.with_chunks = a->top > 0;
   P.T.heads = static_cast<TileHead*>(a->workspace);
   P.T.chunk_max = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + s.chunks_at);
