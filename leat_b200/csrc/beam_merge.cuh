@@ -17,8 +17,9 @@ namespace leat {
 
 constexpr int BM_MAX_BEAMS = 64;
 constexpr int BM_MAX_WIDTH = 64;
-constexpr int BM_LIST = 256;    // nodes a level hands to the next
+constexpr int BM_LIST = 512;    // nodes a level hands to the next
 constexpr int BM_PARTS = 128;   // parts of the block whose best bound a level: at least twice the width
+constexpr int BM_FEW = 16;      // up to this width 32 parts, one per lane, will do
 
 struct MergeParams {
   TileParams T;
@@ -78,6 +79,34 @@ __device__ __forceinline__ LogSum row_log_sum(TileHead h, const TileHead* heads,
   return LogSum{m, plain ? log(s) + ((double)e * ln2_exact - (double)m) - off * (double)m : log(s)};
 }
 
+// the same in float32, to within 2^-19: what the levels below rank by while other warps work out the
+// exact one.  h, more: the lane's headers of the first 64.
+__device__ __forceinline__ LogSum near_log_sum(TileHead h, TileHead more, const TileHead* heads, int tiles, int lane) {
+  constexpr float ln2_float = 0.693147182f, ln2_rest = -1.90465421e-09f, off = -1.3349756e-08f;  // (off: as above)
+  if (lane >= tiles) h.max = neg_inf();
+  if (lane + 32 >= tiles) more.max = neg_inf();
+  float m = fmaxf(h.max, more.max);
+  for (int t = lane + 64; t < tiles; t += 32) m = fmaxf(m, heads[t].max);
+  m = warp_largest(m);
+  if (m == neg_inf()) return LogSum{m, 0.0};
+  const bool plain = fabsf(m) < PLAIN_LIMIT;
+  const float e = plain ? ceilf(m * log2e()) : 0.0f;
+  auto part = [&](const TileHead& v) {
+    if (!(v.max > neg_inf())) return 0.0f;
+    if (!plain || v.exponent == OVER_MAX) return (float)part_beyond(v, m, plain ? (int)e : OVER_MAX);
+    return (float)(v.sum * two_to(v.exponent - (int)e));
+  };
+  float s = part(h) + part(more);
+  for (int t = lane + 64; t < tiles; t += 32) s += part(heads[t]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(FULL, s, d);
+  float log2_s;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(log2_s) : "f"(s));
+  float log = log2_s * ln2_float;
+  if (plain) log += (__fmaf_rn(e, ln2_float, -m) + e * ln2_rest) - off * m;
+  return LogSum{m, (double)log};
+}
+
 template <int FMT>
 __device__ __forceinline__ float one_logit(const void* logits, size_t at) {
   if (FMT == 0) return static_cast<const float*>(logits)[at];
@@ -90,18 +119,22 @@ struct Beam {
   double base;     // score of its likeliest continuation, or of the finished beam
   double divisor;  // the length penalty of its continuations
   float max;       // its largest logit
-  float near_base, near_scale;  // base and 1 / divisor, rounded
   int state;       // 0 dead, 1 live, 2 finished
 };
 // +inf counts as the largest float
 __device__ __forceinline__ double score_of(const Beam& b, float x) {
   return b.base + ((double)fminf(x, largest_float()) - (double)b.max);
 }
-// A rank to within 2^-22 of itself and of the beam's base, enough to leave most logits out: 2 to the
-// -24th for each of the base's, the scale's and the difference's rounding and for the sum's and the
-// product's.  As ordered bits, never 0; 0 for no logit, or a NaN.
-__device__ __forceinline__ unsigned near_rank(const Beam& b, float x) {
-  return x > neg_inf() ? ord32((b.near_base + (x - b.max)) * b.near_scale + 0.0f) : 0u;
+// Ranks to within 2^-21 of themselves and of the beam's reach, scale * (|base| + 8), enough to leave most
+// logits out: 2^-24 for the base's, the scale's and the difference's rounding and for the sum's and the
+// product's, and 2^-19 for the base's own error.  A beam that is not live has a NaN for its base.
+struct __align__(16) Near {
+  float base, max, scale, pad;
+};
+// as ordered bits; 0 for what is no continuation: no logit, a NaN, or a beam that is not live
+__device__ __forceinline__ unsigned near_rank(const Near& b, float x) {
+  const float v = (b.base + (x - b.max)) * b.scale;
+  return x > neg_inf() && v == v ? ord32(v + 0.0f) : 0u;
 }
 
 struct Pick {  // a node, or a logit
@@ -124,33 +157,68 @@ __device__ __forceinline__ bool goes_before(const Node& a, const Node& b) {
   return a.key > b.key;
 }
 
-template <int THREADS>
+// THREADS that go down the levels, EXACT threads behind them, STAGE maxima kept on the chip
+template <int THREADS_, int EXACT_, int STAGE_>
 struct Level {
+  static constexpr int THREADS = THREADS_, EXACT = EXACT_, STAGE = STAGE_;
+  float stage[STAGE];  // the tiles' maxima, if they fit
   Beam beams[BM_MAX_BEAMS];
-  float reach;  // largest |near_base * near_scale| of the beams
+  Near near[BM_MAX_BEAMS];
+  float reach;  // largest scale * (|base| + 8) of the live beams
   Pick list[2][BM_LIST];
-  unsigned part_best[BM_PARTS];
+  __align__(16) unsigned part_best[BM_PARTS];
   int found[2];  // (one per list: a slow thread may still read one while the next level clears the other)
   Node warp_best[THREADS / 32];
-  Pick warp_pick[THREADS / 32];
 };
 
-// The `want` best nodes, one after the other: what best_nodes comes to where its list would overflow
-template <int THREADS, typename Each>
-__device__ __noinline__ void one_by_one(Level<THREADS>& L, int which, int n, int want, Each each) {
-  constexpr int WARPS = THREADS / 32;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// Of a block, the first Level::THREADS threads go down the levels; behind them are warps that meanwhile
+// work out the beams' exact bases, which take three times as long as the float32 ones.  A barrier of
+// the former, and the one place where they wait for the latter, who only arrive there.
+constexpr int BARRIER_LEVELS = 1, BARRIER_EXACT = 2;
+template <typename Level>
+__device__ __forceinline__ void level_sync() {
+  asm volatile("bar.sync %0, %1;" ::"r"(BARRIER_LEVELS), "r"(Level::THREADS) : "memory");
+}
+template <typename Level>
+__device__ __forceinline__ void wait_for_exact(bool& known) {
+  if (known) return;
+  known = true;
+  asm volatile("bar.sync %0, %1;" ::"r"(BARRIER_EXACT), "r"(Level::THREADS + Level::EXACT) : "memory");
+}
+template <typename Level>
+__device__ __forceinline__ void exact_is_known() {
+  __threadfence_block();
+  asm volatile("bar.arrive %0, %1;" ::"r"(BARRIER_EXACT), "r"(Level::THREADS + Level::EXACT) : "memory");
+}
+
+// A level's nodes come in units of 32, one per lane, of one beam:
+//   beam(u)            the unit's beam
+//   peek(u, k)         the largest logit of the lane's node
+//   token(u, k)        its first token
+//   each(u, k, visit)  calls visit(logit, token) for what the node puts on the list (SELF: the node
+//                      itself; else its logits)
+// Units of beams that are not live hold nothing, but may be read.  There are no branches where a unit is
+// looked at: the block does little else than wait for loads, and a branch between two would have the
+// second wait for the first.
+
+// The `want` best, one after the other: what best_nodes comes to where its list would overflow
+template <typename Level, typename Unit>
+__device__ __noinline__ void one_by_one(Level& L, int which, int units, int want, Unit unit) {
+  constexpr int WARPS = Level::THREADS / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Node last{0.0, 0ull, -1};
 #pragma unroll 1
   for (int r = 0; r < want; ++r) {
     Node mine{0.0, 0ull, -1};
 #pragma unroll 1
-    for (int i = tid; i < n; i += THREADS)
-      each(i, [&](float x, int k, int token) {
-        if (!(x > neg_inf())) return;
+    for (int u = warp; u < units; u += WARPS) {
+      const int k = unit.beam(u);
+      unit.each(u, k, [&](float x, int token) {
+        if (near_rank(L.near[k], x) == 0u) return;
         const Node v = node_of(L.beams, Pick{x, token, k});
         if ((last.beam < 0 || goes_before(last, v)) && (mine.beam < 0 || goes_before(v, mine))) mine = v;
       });
+    }
     __syncwarp();
 #pragma unroll 1
     for (int d = 16; d > 0; d >>= 1) {
@@ -161,7 +229,7 @@ __device__ __noinline__ void one_by_one(Level<THREADS>& L, int which, int n, int
       if (o.beam >= 0 && (mine.beam < 0 || goes_before(o, mine))) mine = o;
     }
     if (lane == 0) L.warp_best[warp] = mine;
-    __syncthreads();
+    level_sync<Level>();
     mine = L.warp_best[0];
 #pragma unroll 1
     for (int w = 1; w < WARPS; ++w) {
@@ -169,54 +237,70 @@ __device__ __noinline__ void one_by_one(Level<THREADS>& L, int which, int n, int
       if (o.beam >= 0 && (mine.beam < 0 || goes_before(o, mine))) mine = o;
     }
     last = mine;  // (there is one: more than `want` were found)
-    if (tid == 0) L.list[which][r] = Pick{key_value(last.key), key_id(last.key), last.beam};
-    __syncthreads();
+    if (threadIdx.x == 0) L.list[which][r] = Pick{key_value(last.key), key_id(last.key), last.beam};
+    level_sync<Level>();
   }
 }
 
-// The `want` best of n nodes, and possibly a few more, into L.list[which], in no order; returns how
-// many.  Every part of the block takes its best near rank, and each warp finds, by bisection, a bound
-// that at least `want` of the parts reach; what is not clearly below it goes on the list.  If that is
-// more than the list holds (equal ranks, most of all), the nodes are taken one after the other.
-//   peek(i, beam): node i's largest logit, and its beam
-//   each(i, visit): calls visit(logit, beam, first token) for what node i puts on the list: itself,
-//                   or, at the last level, its logits
-template <int THREADS, typename Peek, typename Each>
-__device__ __forceinline__ int best_nodes(Level<THREADS>& L, int which, int n, int want, Peek peek, Each each) {
-  constexpr int LANES = THREADS / BM_PARTS, AHEAD = 4, PER_LANE = BM_PARTS / 32;
-  const int tid = threadIdx.x, lane = tid & 31;
-  unsigned first[AHEAD];  // of the thread's first nodes: usually all it has
-  unsigned best = 0u;
-  auto look = [&](int base, unsigned (&bits)[AHEAD]) {
+// The `want` best nodes, and possibly a few more, into L.list[which], in no order; returns how many.
+// Every part of the block takes its best near rank, and each warp finds a bound that at least `want` of
+// the parts reach; what is not clearly below it goes on the list.  If that is more than the list holds
+// (equal ranks, most of all), the nodes are taken one after the other.
+template <typename Level, typename Unit>
+__device__ __forceinline__ int best_nodes(Level& L, int which, int units, int want, Unit unit, bool& known) {
+  constexpr int THREADS = Level::THREADS, WARPS = THREADS / 32, AHEAD = 4, PER_LANE = BM_PARTS / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (units == 0) return 0;
+  // 32 parts, one per lane of who compares them, where that makes enough; else BM_PARTS
+  const bool few = want <= BM_FEW && min(units, WARPS) * (32 / WARPS) >= want;
+  struct Batch {
     float x[AHEAD];
-    int beam[AHEAD];
+    int k[AHEAD];
+    unsigned bits[AHEAD];
+  };
+  auto look = [&](int base, Batch& b) {
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      const int i = base + a * THREADS + tid;
-      x[a] = neg_inf();
-      beam[a] = 0;
-      if (i < n) x[a] = peek(i, beam[a]);
+      const int u = min(base + a * WARPS, units - 1);
+      b.k[a] = unit.beam(u);
+      b.x[a] = unit.peek(u, b.k[a]);
     }
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a) bits[a] = near_rank(L.beams[beam[a]], x[a]);
+    for (int a = 0; a < AHEAD; ++a) b.bits[a] = base + a * WARPS < units ? near_rank(L.near[b.k[a]], b.x[a]) : 0u;
   };
-  look(0, first);
-#pragma unroll
-  for (int a = 0; a < AHEAD; ++a) best = max(best, first[a]);
+  Batch first;  // usually all that the warp has
+  look(warp, first);
+  unsigned best = max(max(first.bits[0], first.bits[1]), max(first.bits[2], first.bits[3]));
 #pragma unroll 1
-  for (int base = THREADS * AHEAD; base < n; base += THREADS * AHEAD) {
-    unsigned bits[AHEAD];
-    look(base, bits);
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a) best = max(best, bits[a]);
+  for (int base = warp + WARPS * AHEAD; base < units; base += WARPS * AHEAD) {
+    Batch b;
+    look(base, b);
+    best = max(best, max(max(b.bits[0], b.bits[1]), max(b.bits[2], b.bits[3])));
   }
+  unsigned at_least;  // 0: fewer parts than wanted have any
+  if (few) {
+    constexpr int LANES = THREADS / 32;
 #pragma unroll
-  for (int d = 1; d < LANES; d *= 2) best = max(best, __shfl_xor_sync(FULL, best, d));
-  if (tid % LANES == 0) L.part_best[tid / LANES] = best;
-  if (tid == 0) L.found[which] = 0;
-  __syncthreads();
-  unsigned bound;
-  {
+    for (int d = 1; d < LANES; d *= 2) best = max(best, __shfl_xor_sync(FULL, best, d));
+    // (the part's number in the last bits, cut off again below: no two are equal)
+    if (tid % LANES == 0) L.part_best[tid / LANES] = (best & ~31u) | (unsigned)(tid / LANES);
+    if (tid == 0) L.found[which] = 0;
+    level_sync<Level>();
+    const unsigned mine = L.part_best[lane];
+    int before = 0;
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(&L.part_best[j]);
+      before += (o.x > mine ? 1 : 0) + (o.y > mine ? 1 : 0) + (o.z > mine ? 1 : 0) + (o.w > mine ? 1 : 0);
+    }
+    at_least = __shfl_sync(FULL, mine, __ffs(__ballot_sync(FULL, before == want - 1)) - 1) & ~31u;
+  } else {
+    constexpr int LANES = THREADS / BM_PARTS;
+#pragma unroll
+    for (int d = 1; d < LANES; d *= 2) best = max(best, __shfl_xor_sync(FULL, best, d));
+    if (tid % LANES == 0) L.part_best[tid / LANES] = best;
+    if (tid == 0) L.found[which] = 0;
+    level_sync<Level>();
     unsigned v[PER_LANE], hi = 0u, lo = 0xFFFFFFFFu;
 #pragma unroll
     for (int j = 0; j < PER_LANE; ++j) {
@@ -237,128 +321,167 @@ __device__ __forceinline__ int best_nodes(Level<THREADS>& L, int which, int n, i
       if (c >= want) lo = mid; else hi = mid;
       if (c >= want && c <= enough) break;
     }
-    bound = 1u;  // (0: fewer parts than wanted have any; all nodes are taken)
-    if (lo > 0u) {
-      const float b = unord32(lo);
-      if (b > neg_inf()) bound = ord32(b - 9.5367431640625e-07f * (fabsf(b) + L.reach) + 0.0f);  // 2^-20: both sides' errors
-    }
+    at_least = lo;
   }
-  auto put = [&](float x, int k, int token) {
-    if (near_rank(L.beams[k], x) >= bound) {
-      const int at = atomicAdd(&L.found[which], 1);
-      if (at < BM_LIST) L.list[which][at] = Pick{x, token, k};
+  unsigned bound = 1u;
+  if (at_least > 0u) {
+    const float b = unord32(at_least);
+    if (b > neg_inf()) bound = ord32(b - 9.5367431640625e-07f * (fabsf(b) + L.reach) + 0.0f);  // 2^-20: both sides' errors
+  }
+  auto collect = [&](int base, const Batch& b) {
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const unsigned hits = __ballot_sync(FULL, b.bits[a] >= bound);
+      if (hits == 0u) continue;
+      const int u = base + a * WARPS, k = b.k[a];
+      if (Unit::SELF) {
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&L.found[which], __popc(hits));
+        at = __shfl_sync(FULL, at, 0) + __popc(hits & ((1u << lane) - 1u));
+        if ((hits >> lane & 1u) && at < BM_LIST) L.list[which][at] = Pick{b.x[a], unit.token(u, k), k};
+      } else if (hits >> lane & 1u) {
+        const Near near = L.near[k];
+        unit.each(u, k, [&](float x, int token) {
+          if (near_rank(near, x) >= bound) {
+            const int at = atomicAdd(&L.found[which], 1);
+            if (at < BM_LIST) L.list[which][at] = Pick{x, token, k};
+          }
+        });
+      }
     }
   };
+  collect(warp, first);
 #pragma unroll 1
-  for (int base = 0; base < n; base += THREADS * AHEAD) {
-    unsigned bits[AHEAD];
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a) bits[a] = first[a];
-    if (base > 0) look(base, bits);
-    unsigned hits = 0u;
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a) hits |= (bits[a] >= bound ? 1u : 0u) << a;
-#pragma unroll 1
-    while (hits) {
-      const int a = __ffs(hits) - 1;
-      hits &= hits - 1u;
-      each(base + a * THREADS + tid, put);
-    }
+  for (int base = warp + WARPS * AHEAD; base < units; base += WARPS * AHEAD) {
+    Batch b;
+    look(base, b);
+    collect(base, b);
   }
-  __syncthreads();
+  level_sync<Level>();
   const int found = L.found[which];
   if (found <= BM_LIST) return found;
-  one_by_one<THREADS>(L, which, n, want, each);
+  wait_for_exact<Level>(known);
+  one_by_one(L, which, units, want, unit);
   return want;
 }
 
-// The `want` best continuations of a group's live rows (and possibly a few more) into L.list[0];
-// returns how many.  VEC as for the tiles.
-template <int THREADS, int FMT, bool VEC>
-__device__ __forceinline__ int best_of_rows(Level<THREADS>& L, const TileParams& T, int row0, int rows, int want) {
-  constexpr int PER = FMT == 0 ? 4 : 8, CHUNK = 32 * PER, TILE = BT_CHUNKS * CHUNK;
-  const int tiles = T.tiles;
-  const TileHead* heads = T.heads + (size_t)row0 * tiles;
-  const float* chunk_max = T.chunk_max + (size_t)row0 * tiles * BT_CHUNKS;
-  auto itself = [](auto peek, auto token_of) {
-    return [=](int i, auto&& visit) {
-      int k;
-      const float x = peek(i, k);
-      visit(x, k, token_of(i, k));
-    };
-  };
-  // tiles, unless there are so few that their chunks may as well be looked at
-  int n = rows * tiles;
-  const bool narrow = n > 2 * want && n * (long long)BT_CHUNKS > 4 * THREADS;
-  if (narrow) {
-    auto peek = [=, &L](int i, int& k) {
-      k = i / tiles;
-      return L.beams[k].state == 1 ? heads[i].max : neg_inf();
-    };
-    auto token_of = [=](int i, int k) { return (i - k * tiles) * TILE; };
-    n = best_nodes<THREADS>(L, 0, n, want, peek, itself(peek, token_of));
+// Where the levels begin: at the chunks of all tiles, where those make one unit for each warp's turn; at
+// the tiles, their maxima left on the chip by the warps that sum rows, or read where they lie.
+enum { FROM_TILES, FROM_STAGED_TILES, FROM_CHUNKS };
+template <typename Level>
+__device__ __forceinline__ int start_of(const Level&, int cells) {
+  return cells <= Level::THREADS / 32 * 4 ? FROM_CHUNKS : (cells <= Level::STAGE ? FROM_STAGED_TILES : FROM_TILES);
+}
+
+// 32 tiles of a row (STAGED: their maxima are in the block's stage)
+template <int FMT, bool STAGED, typename Level>
+struct TileUnit {
+  static constexpr bool SELF = true;
+  Level& L;
+  const TileHead* heads;
+  int tiles, per_row;
+  __device__ __forceinline__ int place(int u, int k) const { return (u - k * per_row) * 32 + (threadIdx.x & 31); }
+  __device__ __forceinline__ int beam(int u) const { return u / per_row; }
+  __device__ __forceinline__ float peek(int u, int k) const {
+    const int t = place(u, k), at = min(t, tiles - 1);
+    const float x = STAGED ? L.stage[k * tiles + at] : heads[(size_t)k * tiles + at].max;
+    return t < tiles ? x : neg_inf();
   }
-  {
-    auto place = [=, &L](int i, int& k) {  // chunk of the group (below 2^31: checked on the host)
-      const int t = i / BT_CHUNKS, c = i % BT_CHUNKS;
-      if (!narrow) {
-        k = t / tiles;
-        return i;
-      }
-      k = L.list[0][t].beam;
-      return (k * tiles + L.list[0][t].token / TILE) * BT_CHUNKS + c;
-    };
-    auto peek = [=, &L](int i, int& k) {
-      const int at = place(i, k);
-      return L.beams[k].state == 1 ? chunk_max[at] : neg_inf();
-    };
-    auto token_of = [=](int i, int) {
-      int k;
-      const int at = place(i, k);
-      return (at - k * tiles * BT_CHUNKS) * CHUNK;
-    };
-    n = best_nodes<THREADS>(L, 1, n * BT_CHUNKS, want, peek, itself(peek, token_of));
+  __device__ __forceinline__ int token(int u, int k) const { return place(u, k) * tile_logits(FMT != 0); }
+  template <typename Visit>
+  __device__ __forceinline__ void each(int u, int k, Visit&& visit) const {
+    visit(peek(u, k), token(u, k));
   }
-  // a node is 16 bytes of a chunk; it puts its logits on the list
-  auto load = [=, &L, &T](int i, int& k, int& token, uint32_t (&w)[4]) {
-    const Pick& chunk = L.list[1][i / 32];
-    k = chunk.beam;
-    token = chunk.token + (i % 32) * PER;
-    const size_t at = (size_t)(row0 + k) * T.row_stride + token;
-    const uint32_t none = FMT == 0 ? 0xFF800000u : (FMT == 1 ? 0xFF80FF80u : 0xFC00FC00u);
-    w[0] = w[1] = w[2] = w[3] = none;
+};
+// the 32 chunks of a tile: of all the group's tiles, or of those on the list
+template <int FMT, bool ALL, typename Level>
+struct ChunkUnit {
+  static constexpr bool SELF = true;
+  static constexpr int TILE = tile_logits(FMT != 0), CHUNK = chunk_logits(FMT != 0);
+  Level& L;
+  const float* chunk_max;
+  int tiles;
+  __device__ __forceinline__ int beam(int u) const { return ALL ? u / tiles : L.list[0][u].beam; }
+  __device__ __forceinline__ float peek(int u, int k) const {
+    const size_t cell = ALL ? (size_t)u : (size_t)k * tiles + L.list[0][u].token / TILE;
+    return chunk_max[cell * BT_CHUNKS + (threadIdx.x & 31)];
+  }
+  __device__ __forceinline__ int token(int u, int k) const {
+    return (ALL ? (u - k * tiles) * TILE : L.list[0][u].token) + (int)(threadIdx.x & 31) * CHUNK;
+  }
+  template <typename Visit>
+  __device__ __forceinline__ void each(int u, int k, Visit&& visit) const {
+    visit(peek(u, k), token(u, k));
+  }
+};
+// the 32 vectors of a chunk on the list, which put their logits on the next
+template <int FMT, bool VEC, typename Level>
+struct VectorUnit {
+  static constexpr bool SELF = false;
+  static constexpr int PER = FMT == 0 ? 4 : 8;
+  Level& L;
+  const void* logits;
+  long long row0, row_stride;
+  int vocab;
+  __device__ __forceinline__ int beam(int u) const { return L.list[1][u].beam; }
+  __device__ __forceinline__ int token(int u, int) const { return L.list[1][u].token + (int)(threadIdx.x & 31) * PER; }
+  __device__ __forceinline__ void load(int u, int k, uint32_t (&w)[4]) const {
+    constexpr uint32_t none = FMT == 0 ? 0xFF800000u : (FMT == 1 ? 0xFF80FF80u : 0xFC00FC00u);
+    const int first = token(u, k);
+    const size_t row = (size_t)(row0 + k) * row_stride;
     if (VEC) {
-      if (token < T.vocab) {
-        const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const char*>(T.logits) + at * (FMT == 0 ? 4 : 2));
-        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-      }
+      const size_t at = row + min(first, vocab - PER);
+      const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const char*>(logits) + at * (FMT == 0 ? 4 : 2));
+      const bool in = first < vocab;
+      w[0] = in ? v.x : none; w[1] = in ? v.y : none; w[2] = in ? v.z : none; w[3] = in ? v.w : none;
     } else if (FMT == 0) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (token + q < T.vocab) w[q] = static_cast<const uint32_t*>(T.logits)[at + q];
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t v = static_cast<const uint32_t*>(logits)[row + min(first + q, vocab - 1)];
+        w[q] = first + q < vocab ? v : none;
+      }
     } else {
 #pragma unroll
-      for (int q = 0; q < 8; ++q)
-        if (token + q < T.vocab) {
-          const uint32_t v = static_cast<const unsigned short*>(T.logits)[at + q];
-          w[q >> 1] = (q & 1) ? (w[q >> 1] & 0xFFFFu) | (v << 16) : (w[q >> 1] & 0xFFFF0000u) | v;
-        }
+      for (int q = 0; q < 8; q += 2) {
+        const unsigned short* const at = static_cast<const unsigned short*>(logits) + row;
+        const uint32_t a = at[min(first + q, vocab - 1)], b = at[min(first + q + 1, vocab - 1)];
+        w[q >> 1] = (first + q < vocab ? a : none & 0xFFFFu) | (first + q + 1 < vocab ? b << 16 : none & 0xFFFF0000u);
+      }
     }
-  };
-  auto peek = [=](int i, int& k) {
-    int token;
+  }
+  __device__ __forceinline__ float peek(int u, int k) const {
     uint32_t w[4];
-    load(i, k, token, w);
+    load(u, k, w);
     return largest_of<FMT>(w[0], w[1], w[2], w[3]);
-  };
-  auto each = [=](int i, auto&& visit) {
-    int k, token;
+  }
+  template <typename Visit>
+  __device__ __forceinline__ void each(int u, int k, Visit&& visit) const {
     uint32_t w[4];
-    load(i, k, token, w);
+    load(u, k, w);
+    const int first = token(u, k);
 #pragma unroll
-    for (int q = 0; q < PER; ++q) visit(held<FMT>(w, q), k, token + q);
-  };
-  return best_nodes<THREADS>(L, 0, n * 32, want, peek, each);
+    for (int q = 0; q < PER; ++q) visit(held<FMT>(w, q), first + q);
+  }
+};
+
+// The `want` best continuations of a group's live rows (and possibly a few more) into L.list[0];
+// returns how many.  VEC as for the tiles.
+template <int FMT, bool VEC, typename Level>
+__device__ __forceinline__ int best_of_rows(Level& L, const TileParams& T, int row0, int rows, int want, int start, bool& known) {
+  const size_t cell0 = (size_t)row0 * T.tiles;
+  const float* chunk_max = T.chunk_max + cell0 * BT_CHUNKS;
+  int n;
+  if (start == FROM_CHUNKS) {
+    n = best_nodes(L, 1, rows * T.tiles, want, ChunkUnit<FMT, true, Level>{L, chunk_max, T.tiles}, known);
+  } else {
+    const int per_row = (T.tiles + 31) / 32;
+    if (start == FROM_STAGED_TILES)
+      n = best_nodes(L, 0, rows * per_row, want, TileUnit<FMT, true, Level>{L, T.heads + cell0, T.tiles, per_row}, known);
+    else
+      n = best_nodes(L, 0, rows * per_row, want, TileUnit<FMT, false, Level>{L, T.heads + cell0, T.tiles, per_row}, known);
+    n = best_nodes(L, 1, n, want, ChunkUnit<FMT, false, Level>{L, chunk_max, T.tiles}, known);
+  }
+  return best_nodes(L, 0, n, want, VectorUnit<FMT, VEC, Level>{L, T.logits, row0, T.row_stride, T.vocab}, known);
 }
 
 // the length penalty: ((5 + length) / 6)^alpha
@@ -366,15 +489,25 @@ __device__ __noinline__ double length_divisor(int length, float alpha) {
   return pow((5.0 + (double)max(length, 0)) / 6.0, (double)alpha);
 }
 
-// one block per group
+// a rank as ordered bits, so that candidates compare as whole numbers
+__device__ __forceinline__ unsigned long long ord64(double r) {
+  const unsigned long long b = (unsigned long long)__double_as_longlong(r + 0.0);
+  return b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
+}
+
+constexpr int BM_EXACT = 256;
+
+// one block per group: THREADS for the levels and BM_EXACT more
 template <int THREADS, int FMT, bool VEC>
-__global__ void __launch_bounds__(THREADS) beam_merge_kernel(const MergeParams P) {
-  constexpr int WARPS = THREADS / 32;
-  __shared__ Level<THREADS> L;
-  __shared__ Node candidates[BM_LIST + BM_MAX_BEAMS];
+__global__ void __launch_bounds__(THREADS + BM_EXACT) beam_merge_kernel(const MergeParams P) {
+  using GroupLevel = Level<THREADS, BM_EXACT, 4096>;
+  __shared__ GroupLevel L;
+  __shared__ unsigned long long ranks[BM_LIST + BM_MAX_BEAMS], keys[BM_LIST + BM_MAX_BEAMS];
+  __shared__ int owners[BM_LIST + BM_MAX_BEAMS];
   __shared__ int finished_n;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, tiles = P.T.tiles;
   const int group = blockIdx.x, row0 = group * P.beams;
+  const int start = start_of(L, P.beams * tiles);
   if (tid == 0) {
     L.reach = 0.0f;
     finished_n = 0;
@@ -382,51 +515,84 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(const MergeParams P
   __syncthreads();
   grid_dependency_wait();
   grid_launch_dependents();
-  for (int k = warp; k < P.beams; k += WARPS) {
-    // (a row's first headers are asked for with its score; those of a row that is not live hold nothing)
-    const TileHead* heads = P.T.heads + (size_t)(row0 + k) * P.T.tiles;
-    TileHead h = {neg_inf(), 0, 0.0};
-    if (lane < P.T.tiles) h = heads[lane];
+  if (tid >= THREADS) {
+    for (int k = warp - THREADS / 32; k < P.beams; k += BM_EXACT / 32) {
+      // (a row's first headers are asked for with its score; those of a row that is not live hold nothing)
+      const TileHead* heads = P.T.heads + (size_t)(row0 + k) * tiles;
+      const TileHead h = heads[min(lane, tiles - 1)];
+      const float score = P.T.scores[row0 + k];
+      const bool done = P.T.finished && P.T.finished[row0 + k], sound = fabsf(score) <= largest_float();
+      LogSum sum = {0.0f, 0.0};
+      if (sound && !done) sum = row_log_sum(h, heads, tiles, lane);
+      if (lane == 0) {
+        const double divisor = P.length_penalty == 0.0f ? 1.0 : length_divisor(P.lengths[row0 + k] + (done ? 0 : 1), P.length_penalty);
+        L.beams[k] = Beam{(double)score - sum.log, divisor, sum.max, !sound ? 0 : (done ? 2 : 1)};
+      }
+    }
+    exact_is_known<GroupLevel>();
+    return;
+  }
+  for (int k = warp; k < P.beams; k += THREADS / 32) {
+    const TileHead* heads = P.T.heads + (size_t)(row0 + k) * tiles;
+    const TileHead h = heads[min(lane, tiles - 1)], more = heads[min(lane + 32, tiles - 1)];
     const float score = P.T.scores[row0 + k];
-    const bool done = P.T.finished && P.T.finished[row0 + k];
-    const bool live = fabsf(score) <= largest_float() && !done;
-    LogSum sum = {0.0f, 0.0};
-    if (live) sum = row_log_sum(h, heads, P.T.tiles, lane);
+    const bool live = fabsf(score) <= largest_float() && !(P.T.finished && P.T.finished[row0 + k]);
+    const int length = P.length_penalty != 0.0f ? P.lengths[row0 + k] + 1 : 0;
+    LogSum sum = {neg_inf(), 0.0};
+    if (live) sum = near_log_sum(h, more, heads, tiles, lane);
+    if (start == FROM_STAGED_TILES) {
+      if (lane < tiles) L.stage[k * tiles + lane] = h.max;
+      if (lane + 32 < tiles) L.stage[k * tiles + lane + 32] = more.max;
+      for (int t = lane + 64; t < tiles; t += 32) L.stage[k * tiles + t] = heads[t].max;
+    }
     if (lane == 0) {
-      Beam b;
-      b.base = (double)score - sum.log;
-      b.max = sum.max;
-      b.state = live && sum.max > neg_inf() ? 1 : (done && fabsf(score) <= largest_float() ? 2 : 0);
-      b.divisor = P.length_penalty == 0.0f ? 1.0 : length_divisor(P.lengths[row0 + k] + (done ? 0 : 1), P.length_penalty);
-      b.near_base = (float)b.base;
-      b.near_scale = (float)(1.0 / b.divisor);
-      L.beams[k] = b;
-      if (b.state == 1) atomicMax(reinterpret_cast<int*>(&L.reach), __float_as_int(fabsf(b.near_base * b.near_scale)));
+      const float base = score - (float)sum.log;
+      const float scale = P.length_penalty == 0.0f ? 1.0f : (float)(1.0 / length_divisor(length, P.length_penalty));
+      const bool any = sum.max > neg_inf();
+      L.near[k] = Near{any ? base : quiet_nan(), sum.max, scale, 0.0f};
+      if (any) atomicMax(reinterpret_cast<int*>(&L.reach), __float_as_int(scale * (fabsf(base) + 8.0f)));
     }
   }
-  __syncthreads();
-  const int live_n = best_of_rows<THREADS, FMT, VEC>(L, P.T, row0, P.beams, P.width);
-  for (int i = tid; i < live_n; i += THREADS) candidates[i] = node_of(L.beams, L.list[0][i]);
+  level_sync<GroupLevel>();
+  bool known = false;
+  const int live_n = best_of_rows<FMT, VEC>(L, P.T, row0, P.beams, P.width, start, known);
+  wait_for_exact<GroupLevel>(known);
+  for (int i = tid; i < live_n; i += THREADS) {
+    const Pick p = L.list[0][i];
+    const Node v = node_of(L.beams, p);
+    ranks[i] = ord64(v.rank);
+    keys[i] = v.key;
+    owners[i] = v.beam;
+  }
   if (P.T.finished)
     for (int k = tid; k < P.beams; k += THREADS)
-      if (L.beams[k].state == 2)
-        candidates[live_n + atomicAdd(&finished_n, 1)] = Node{L.beams[k].base / L.beams[k].divisor, make_key(0.0f, (uint32_t)P.end_id), k};
-  __syncthreads();
+      if (L.beams[k].state == 2) {
+        const int i = live_n + atomicAdd(&finished_n, 1);
+        ranks[i] = ord64(L.beams[k].base / L.beams[k].divisor);
+        keys[i] = make_key(0.0f, (uint32_t)P.end_id);
+        owners[i] = k;
+      }
+  level_sync<GroupLevel>();
   const int all = live_n + finished_n;
   for (int i = tid; i < all; i += THREADS) {
-    const Node c = candidates[i];
+    const unsigned long long rank = ranks[i], key = keys[i];
+    const int beam = owners[i];
     int before = 0;
-    for (int j = 0; j < all; ++j) before += goes_before(candidates[j], c) ? 1 : 0;
+#pragma unroll 4
+    for (int j = 0; j < all; ++j) {
+      const unsigned long long r = ranks[j];
+      before += r > rank || (r == rank && (owners[j] < beam || (owners[j] == beam && keys[j] > key))) ? 1 : 0;
+    }
     if (before >= P.width) continue;
     const size_t at = (size_t)group * P.width + before;
-    const int token = key_id(c.key);
-    const Beam& b = L.beams[c.beam];
+    const int token = key_id(key);
+    const Beam& b = L.beams[beam];
     const bool was = b.state == 2;
     P.out_tokens[at] = token;
-    P.out_parents[at] = c.beam;
-    P.out_scores[at] = (float)(was ? b.base : score_of(b, key_value(c.key)));
+    P.out_parents[at] = beam;
+    P.out_scores[at] = (float)(was ? b.base : score_of(b, key_value(key)));
     if (P.out_finished) P.out_finished[at] = was || token == P.end_id ? 1 : 0;
-    if (P.out_lengths) P.out_lengths[at] = P.lengths[row0 + c.beam] + (was ? 0 : 1);
+    if (P.out_lengths) P.out_lengths[at] = P.lengths[row0 + beam] + (was ? 0 : 1);
   }
   // places without a continuation: no token, no score, the beam of the place itself as parent
   for (int j = min(all, P.width) + tid; j < P.width; j += THREADS) {
@@ -440,38 +606,50 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(const MergeParams P
 }
 
 constexpr int LP_THREADS = 128;
+constexpr int LP_EXACT = 32;
 
-// one block per row
+// one block per row: a warp for the exact sum and the given ids, the others for the likeliest
 template <int FMT, bool VEC>
-__global__ void __launch_bounds__(LP_THREADS) logprob_kernel(const LogprobParams P) {
-  __shared__ Level<LP_THREADS> L;
+__global__ void __launch_bounds__(LP_THREADS + LP_EXACT) logprob_kernel(const LogprobParams P) {
+  using RowLevel = Level<LP_THREADS, LP_EXACT, 1>;
+  __shared__ RowLevel L;
   __shared__ unsigned long long keys[BM_LIST];
-  const int tid = threadIdx.x, lane = tid & 31, row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, row = blockIdx.x, tiles = P.T.tiles;
+  const TileHead* heads = P.T.heads + (size_t)row * tiles;
   grid_dependency_wait();
   grid_launch_dependents();
-  const TileHead* heads = P.T.heads + (size_t)row * P.T.tiles;
-  TileHead h = {neg_inf(), 0, 0.0};
-  if (lane < P.T.tiles) h = heads[lane];
-  const LogSum sum = row_log_sum(h, heads, P.T.tiles, lane);
-  const Beam own{-sum.log, 1.0, sum.max, (float)-sum.log, 1.0f, sum.max > neg_inf() ? 1 : 0};
-  for (int g = tid; g < P.given; g += LP_THREADS) {
-    const int id = P.ids[(size_t)row * P.given + g];
-    float x = neg_inf();  // ids outside the vocabulary have probability zero
-    if (id >= 0 && id < P.T.vocab) x = one_logit<FMT>(P.T.logits, (size_t)row * P.T.row_stride + id);
-    P.out_given[(size_t)row * P.given + g] = x > neg_inf() ? (float)score_of(own, x) : neg_inf();  // (NaN as -inf)
+  if (tid >= LP_THREADS) {
+    const LogSum sum = row_log_sum(heads[min(lane, tiles - 1)], heads, tiles, lane);
+    const Beam own{-sum.log, 1.0, sum.max, 1};
+    if (lane == 0) L.beams[0] = own;
+    exact_is_known<RowLevel>();
+    for (int g = lane; g < P.given; g += 32) {
+      const int id = P.ids[(size_t)row * P.given + g];
+      float x = neg_inf();  // ids outside the vocabulary have probability zero
+      if (id >= 0 && id < P.T.vocab) x = one_logit<FMT>(P.T.logits, (size_t)row * P.T.row_stride + id);
+      P.out_given[(size_t)row * P.given + g] = x > neg_inf() ? (float)score_of(own, x) : neg_inf();  // (NaN as -inf)
+    }
+    return;
   }
-  if (P.top == 0) return;
-  if (tid == 0) {
-    L.beams[0] = own;
-    L.reach = fabsf(own.near_base);
+  const int start = start_of(L, tiles) == FROM_CHUNKS ? FROM_CHUNKS : FROM_TILES;
+  if (tid < 32) {
+    const LogSum sum = near_log_sum(heads[min(lane, tiles - 1)], heads[min(lane + 32, tiles - 1)], heads, tiles, lane);
+    if (lane == 0) {
+      L.near[0] = Near{sum.max > neg_inf() ? -(float)sum.log : quiet_nan(), sum.max, 1.0f, 0.0f};
+      L.reach = fabsf((float)sum.log) + 8.0f;
+    }
   }
-  __syncthreads();
-  const int all = best_of_rows<LP_THREADS, FMT, VEC>(L, P.T, row, 1, P.top);
+  level_sync<RowLevel>();
+  bool known = false;
+  const int all = best_of_rows<FMT, VEC>(L, P.T, row, 1, P.top, start, known);
+  wait_for_exact<RowLevel>(known);
   for (int i = tid; i < all; i += LP_THREADS) keys[i] = make_key(L.list[0][i].x, (uint32_t)L.list[0][i].token);
-  __syncthreads();
+  level_sync<RowLevel>();
+  const Beam own = L.beams[0];
   for (int i = tid; i < all; i += LP_THREADS) {
     const unsigned long long key = keys[i];  // (one beam: its keys' order is the order)
     int before = 0;
+#pragma unroll 4
     for (int j = 0; j < all; ++j) before += keys[j] > key ? 1 : 0;
     if (before >= P.top) continue;
     P.out_top[(size_t)row * P.top + before] = (float)score_of(own, key_value(key));
@@ -480,6 +658,29 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_kernel(const LogprobParams
   for (int j = min(all, P.top) + tid; j < P.top; j += LP_THREADS) {
     P.out_top[(size_t)row * P.top + j] = neg_inf();
     P.out_top_ids[(size_t)row * P.top + j] = -1;
+  }
+}
+
+// and where only given ids are asked for: a warp per row
+template <int FMT>
+__global__ void __launch_bounds__(LP_THREADS) given_kernel(const LogprobParams P) {
+  const int lane = threadIdx.x & 31, row = blockIdx.x * (LP_THREADS / 32) + (threadIdx.x >> 5), tiles = P.T.tiles;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  if (row >= P.T.rows) return;
+  const TileHead* heads = P.T.heads + (size_t)row * tiles;
+  const TileHead h = heads[min(lane, tiles - 1)];
+  float first = neg_inf();
+  auto logit = [&](int g) {
+    const int id = P.ids[(size_t)row * P.given + g];
+    return id >= 0 && id < P.T.vocab ? one_logit<FMT>(P.T.logits, (size_t)row * P.T.row_stride + id) : neg_inf();
+  };
+  if (lane < P.given) first = logit(lane);
+  const LogSum sum = row_log_sum(h, heads, tiles, lane);
+  const Beam own{-sum.log, 1.0, sum.max, 1};
+  for (int g = lane; g < P.given; g += 32) {
+    const float x = g < 32 ? first : logit(g);
+    P.out_given[(size_t)row * P.given + g] = x > neg_inf() ? (float)score_of(own, x) : neg_inf();
   }
 }
 

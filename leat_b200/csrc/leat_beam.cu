@@ -18,7 +18,6 @@ namespace {
 
 constexpr int kMaxGroups = 65535;  // a grid's second dimension
 constexpr long long kMaxBlocks = 0x7FFFFFFF;
-constexpr int MERGE_THREADS = 256;
 
 struct Scratch {
   int tiles;
@@ -66,14 +65,19 @@ template <int FMT, bool VEC>
 struct Select {
   static cudaError_t both(const MergeParams& P, int rows, int groups, cudaStream_t stream) {
     const cudaError_t e = Tiles<FMT, VEC>::launch(P.T, rows, stream);
-    return e != cudaSuccess ? e : launch_dependent(beam_merge_kernel<MERGE_THREADS, FMT, VEC>, dim3(groups), dim3(MERGE_THREADS), 0, stream, P);
+    if (e != cudaSuccess) return e;
+    // few continuations: small blocks, whose barriers and bounds cost less; many: more nodes at a time
+    return P.width <= BM_FEW ? launch_dependent(beam_merge_kernel<256, FMT, VEC>, dim3(groups), dim3(256 + BM_EXACT), 0, stream, P)
+                             : launch_dependent(beam_merge_kernel<512, FMT, VEC>, dim3(groups), dim3(512 + BM_EXACT), 0, stream, P);
   }
 };
 template <int FMT, bool VEC>
 struct Logprobs {
   static cudaError_t both(const LogprobParams& P, int rows, int, cudaStream_t stream) {
     const cudaError_t e = Tiles<FMT, VEC>::launch(P.T, rows, stream);
-    return e != cudaSuccess ? e : launch_dependent(logprob_kernel<FMT, VEC>, dim3(rows), dim3(LP_THREADS), 0, stream, P);
+    if (e != cudaSuccess) return e;
+    return P.top > 0 ? launch_dependent(logprob_kernel<FMT, VEC>, dim3(rows), dim3(LP_THREADS + LP_EXACT), 0, stream, P)
+                     : launch_dependent(given_kernel<FMT>, dim3((rows + LP_THREADS / 32 - 1) / (LP_THREADS / 32)), dim3(LP_THREADS), 0, stream, P);
   }
 };
 
