@@ -574,16 +574,22 @@ __global__ void __launch_bounds__(THREADS + BM_EXACT) beam_merge_kernel(const Me
       }
   level_sync<GroupLevel>();
   const int all = live_n + finished_n;
-  for (int i = tid; i < all; i += THREADS) {
+  // each candidate's place: how many go before it, counted by eight lanes
+  for (int i0 = 0; i0 < all; i0 += THREADS / 8) {
+    const int i = min(i0 + tid / 8, all - 1);
     const unsigned long long rank = ranks[i], key = keys[i];
     const int beam = owners[i];
     int before = 0;
-#pragma unroll 4
-    for (int j = 0; j < all; ++j) {
-      const unsigned long long r = ranks[j];
-      before += r > rank || (r == rank && (owners[j] < beam || (owners[j] == beam && keys[j] > key))) ? 1 : 0;
+#pragma unroll 2
+    for (int j = tid & 7; j < all; j += 8) {
+      const unsigned long long r = ranks[j], o = keys[j];
+      const int k = owners[j];
+      before += (r > rank) | ((r == rank) & ((k < beam) | ((k == beam) & (o > key)))) ? 1 : 0;
     }
-    if (before >= P.width) continue;
+    __syncwarp();
+#pragma unroll
+    for (int d = 1; d < 8; d *= 2) before += __shfl_xor_sync(FULL, before, d);
+    if ((tid & 7) != 0 || i0 + tid / 8 >= all || before >= P.width) continue;
     const size_t at = (size_t)group * P.width + before;
     const int token = key_id(key);
     const Beam& b = L.beams[beam];
@@ -646,12 +652,15 @@ __global__ void __launch_bounds__(LP_THREADS + LP_EXACT) logprob_kernel(const Lo
   for (int i = tid; i < all; i += LP_THREADS) keys[i] = make_key(L.list[0][i].x, (uint32_t)L.list[0][i].token);
   level_sync<RowLevel>();
   const Beam own = L.beams[0];
-  for (int i = tid; i < all; i += LP_THREADS) {
-    const unsigned long long key = keys[i];  // (one beam: its keys' order is the order)
+  for (int i0 = 0; i0 < all; i0 += LP_THREADS / 8) {
+    const unsigned long long key = keys[min(i0 + tid / 8, all - 1)];  // (one beam: its keys' order is the order)
     int before = 0;
-#pragma unroll 4
-    for (int j = 0; j < all; ++j) before += keys[j] > key ? 1 : 0;
-    if (before >= P.top) continue;
+#pragma unroll 2
+    for (int j = tid & 7; j < all; j += 8) before += keys[j] > key ? 1 : 0;
+    __syncwarp();
+#pragma unroll
+    for (int d = 1; d < 8; d *= 2) before += __shfl_xor_sync(FULL, before, d);
+    if ((tid & 7) != 0 || i0 + tid / 8 >= all || before >= P.top) continue;
     P.out_top[(size_t)row * P.top + before] = (float)score_of(own, key_value(key));
     P.out_top_ids[(size_t)row * P.top + before] = key_id(key);
   }
