@@ -615,16 +615,16 @@ constexpr int LP_THREADS = 128;
 constexpr int LP_EXACT = 32;
 
 // one block per row: a warp for the exact sum and the given ids, the others for the likeliest
-template <int FMT, bool VEC>
-__global__ void __launch_bounds__(LP_THREADS + LP_EXACT) logprob_kernel(const LogprobParams P) {
-  using RowLevel = Level<LP_THREADS, LP_EXACT, 1>;
+template <int THREADS, int FMT, bool VEC>
+__global__ void __launch_bounds__(THREADS + LP_EXACT) logprob_kernel(const LogprobParams P) {
+  using RowLevel = Level<THREADS, LP_EXACT, 1>;
   __shared__ RowLevel L;
   __shared__ unsigned long long keys[BM_LIST];
   const int tid = threadIdx.x, lane = tid & 31, row = blockIdx.x, tiles = P.T.tiles;
   const TileHead* heads = P.T.heads + (size_t)row * tiles;
   grid_dependency_wait();
   grid_launch_dependents();
-  if (tid >= LP_THREADS) {
+  if (tid >= THREADS) {
     const LogSum sum = row_log_sum(heads[min(lane, tiles - 1)], heads, tiles, lane);
     const Beam own{-sum.log, 1.0, sum.max, 1};
     if (lane == 0) L.beams[0] = own;
@@ -649,10 +649,10 @@ __global__ void __launch_bounds__(LP_THREADS + LP_EXACT) logprob_kernel(const Lo
   bool known = false;
   const int all = best_of_rows<FMT, VEC>(L, P.T, row, 1, P.top, start, known);
   wait_for_exact<RowLevel>(known);
-  for (int i = tid; i < all; i += LP_THREADS) keys[i] = make_key(L.list[0][i].x, (uint32_t)L.list[0][i].token);
+  for (int i = tid; i < all; i += THREADS) keys[i] = make_key(L.list[0][i].x, (uint32_t)L.list[0][i].token);
   level_sync<RowLevel>();
   const Beam own = L.beams[0];
-  for (int i0 = 0; i0 < all; i0 += LP_THREADS / 8) {
+  for (int i0 = 0; i0 < all; i0 += THREADS / 8) {
     const unsigned long long key = keys[min(i0 + tid / 8, all - 1)];  // (one beam: its keys' order is the order)
     int before = 0;
 #pragma unroll 2
@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(LP_THREADS + LP_EXACT) logprob_kernel(const Lo
     P.out_top[(size_t)row * P.top + before] = (float)score_of(own, key_value(key));
     P.out_top_ids[(size_t)row * P.top + before] = key_id(key);
   }
-  for (int j = min(all, P.top) + tid; j < P.top; j += LP_THREADS) {
+  for (int j = min(all, P.top) + tid; j < P.top; j += THREADS) {
     P.out_top[(size_t)row * P.top + j] = neg_inf();
     P.out_top_ids[(size_t)row * P.top + j] = -1;
   }
