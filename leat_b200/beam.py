@@ -14,11 +14,11 @@ from struct import pack
 import torch
 
 from leat_b200 import _lib
-from leat_b200.logprobs import FORMATS, launch, rows_of_logits, scratch
+from leat_b200.logprobs import FORMATS, empty_matrices, empty_matrix, raw_stream, rows_of_logits, scratch
 
 MAX_BEAMS = 64
 MAX_WIDTH = 64
-STATE_WORDS = "PqqqiiiI"  # struct leat_state, with the padding at its end
+STATE_REST = "qqqiiiI"  # struct leat_state behind its address, with the padding at its end
 
 
 @dataclass
@@ -64,6 +64,9 @@ def beam_select(logits, scores: torch.Tensor, width: int | None = None, *, finis
     `out`: a Selected of an earlier call (or of your own contiguous tensors) to write into."""
     logits = rows_of_logits(logits)
     dev = logits.device
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return beam_select(logits, scores, width, finished=finished, end_id=end_id, lengths=lengths, length_penalty=length_penalty, out=out)
     rows, vocab = logits.shape
     if not isinstance(scores, torch.Tensor) or scores.dim() != 2:
         raise ValueError("scores must be a (G, K) float32 tensor")
@@ -93,9 +96,9 @@ def beam_select(logits, scores: torch.Tensor, width: int | None = None, *, finis
     elif length_penalty != 0.0:
         raise ValueError("length_penalty needs the beams' lengths")
     if out is None:
-        tokens, parents, bits, *more = torch.empty(3 if lengths is None else 4, groups, width, dtype=torch.int32, device=dev).unbind(0)
-        out = Selected(tokens, parents, bits.view(torch.float32), None if end_id is None else torch.empty(groups, width, dtype=torch.bool, device=dev),
-                       None if lengths is None else more[0])  # fmt: skip
+        out = Selected(empty_matrix(groups, width, torch.int32), empty_matrix(groups, width, torch.int32), empty_matrix(groups, width, torch.float32),
+                       None if end_id is None else empty_matrix(groups, width, torch.bool),
+                       None if lengths is None else empty_matrix(groups, width, torch.int32))  # fmt: skip
     else:
         wanted = [(out.tokens, torch.int32), (out.parents, torch.int32), (out.scores, torch.float32)]
         wanted += [(out.finished, torch.bool)] if end_id is not None else []
@@ -112,12 +115,14 @@ def beam_select(logits, scores: torch.Tensor, width: int | None = None, *, finis
         ended_at = out.finished.data_ptr()
     if lengths is not None:
         new_lengths_at = out.lengths.data_ptr()
-    held, at, size = scratch(rows, vocab, width, dev)
+    held, at, size = scratch(rows, vocab, width)
     a = _lib.BeamArgs(
         logits.data_ptr(), groups, beams, vocab, width, logits.stride(0), FORMATS[logits.dtype], -1 if end_id is None else end_id,
         scores.data_ptr(), done_at, lengths_at, length_penalty, out.tokens.data_ptr(), out.parents.data_ptr(), out.scores.data_ptr(),
         ended_at, new_lengths_at, at, size)  # fmt: skip
-    launch(dev.index, "leat_beam_select", _lib.lib.leat_beam_select, a)
+    code = _lib.lib.leat_beam_select(a, raw_stream(dev.index))
+    if code != _lib.OK:
+        _lib.check(code, "leat_beam_select")
     return out
 
 
@@ -196,24 +201,29 @@ def reorder_states(states, parents: torch.Tensor, *, slots: torch.Tensor | None 
     states = [states] if isinstance(states, torch.Tensor) else list(states)
     if not isinstance(parents, torch.Tensor) or parents.dim() != 2 or not parents.is_cuda:
         raise ValueError("parents must be a (G, K) int32 CUDA tensor")
-    groups, beams = parents.shape
     dev = parents.device
-    parents = _whole(parents, torch.int32, (groups, beams), dev, "parents")
+    index = dev.index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(dev):
+            return reorder_states(states, parents, slots=slots, dim=dim, start=start, length=length)
+    groups, beams = parents.shape
+    parents = _whole(parents, torch.int32, parents.shape, dev, "parents")
     if not 1 <= beams <= MAX_BEAMS or groups > 65535:
         raise ValueError(f"parents must be (G, K) with K from 1 to {MAX_BEAMS} and G up to 65535")
     if slots is not None:
-        slots = _whole(slots, torch.int32, (groups, beams), dev, "slots")
-    if dim is None and (length is not None or (start is not None and not (isinstance(start, int) and start == 0))):
+        slots = _whole(slots, torch.int32, parents.shape, dev, "slots")
+    if dim is None and (length is not None or (start is not None and (isinstance(start, torch.Tensor) or start != 0))):
         raise ValueError("start and length count positions: say which dimension they are with dim")
     start_at, start_all, keep_start = _range_end(0 if start is None else start, groups, dev, "start")
     end_at, end_all, keep_end = _range_end(0x7FFFFFFF if length is None else length, groups, dev, "length")
     # a search's caches are mostly alike: what one comes to holds for the next of its shape and strides
-    words: list[int] = []
-    index, shape, stride, dtype = dev.index, None, None, None
+    described: list[bytes] = []
+    shape = dtype = stride = None
+    plain = False  # the last was contiguous: the next is alike if it is, too
     for t in states:
         if not isinstance(t, torch.Tensor) or t.get_device() != index or t.requires_grad:
             raise ValueError(f"states must be tensors on {dev}, rows first, that need no gradient")
-        if t.shape != shape or t.dtype != dtype or t.stride() != stride:
+        if t.shape != shape or t.dtype != dtype or not (t.is_contiguous() if plain else t.stride() == stride):
             if t.layout is not torch.strided or t.dim() == 0:
                 raise ValueError("states must be strided tensors with their rows as first dimension")
             if slots is None and t.shape[0] < groups * beams:
@@ -225,13 +235,15 @@ def reorder_states(states, parents: torch.Tensor, *, slots: torch.Tensor | None 
             like = _state(t, dim)
             if _overlaps(*like):
                 raise ValueError("the rows of a state must not overlap")
-            shape, dtype, stride = t.shape, t.dtype, t.stride()
-        words += (t.data_ptr(), *like, 0)
-    if not words or groups == 0:
+            shape, dtype, stride, plain = t.shape, t.dtype, t.stride(), t.is_contiguous()
+            rest = pack(STATE_REST, *like, 0)
+        described.append(pack("P", t.data_ptr()) + rest)
+    if not described or groups == 0:
         return
-    count = len(words) // 8
-    launch(index, "leat_reorder_states", _lib.lib.leat_reorder_states, pack(STATE_WORDS * count, *words), count, parents.data_ptr(),
-           None if slots is None else slots.data_ptr(), groups, beams, start_at, start_all, end_at, end_all)  # fmt: skip
+    code = _lib.lib.leat_reorder_states(b"".join(described), len(described), parents.data_ptr(), None if slots is None else slots.data_ptr(),
+                                        groups, beams, start_at, start_all, end_at, end_all, raw_stream(index))  # fmt: skip
+    if code != _lib.OK:
+        _lib.check(code, "leat_reorder_states")
     del keep_start, keep_end
 
 
@@ -241,19 +253,23 @@ def beam_sequences(tokens: torch.Tensor, parents: torch.Tensor, end_id: int | No
     sequence's length ends with its first end token, and only end tokens stand behind it."""
     if not isinstance(tokens, torch.Tensor) or tokens.dim() != 3 or not tokens.is_cuda:
         raise ValueError("tokens must be a (T, G, K) int32 CUDA tensor")
-    steps, groups, beams = tokens.shape
     dev = tokens.device
-    tokens = _whole(tokens, torch.int32, (steps, groups, beams), dev, "tokens")
-    parents = _whole(parents, torch.int32, (steps, groups, beams), dev, "parents")
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return beam_sequences(tokens, parents, end_id)
+    steps, groups, beams = shape = tokens.shape
+    tokens = _whole(tokens, torch.int32, shape, dev, "tokens")
+    parents = _whole(parents, torch.int32, shape, dev, "parents")
     if not 1 <= beams <= MAX_BEAMS:
         raise ValueError(f"there must be 1 to {MAX_BEAMS} beams")
     if end_id is not None and (isinstance(end_id, bool) or not isinstance(end_id, int) or not 0 <= end_id <= 0x7FFFFFFF):
         raise ValueError("end_id must be a token")
-    out = Sequences(torch.empty(groups, beams, steps, dtype=torch.int32, device=dev),
-                    torch.empty(groups, beams, dtype=torch.int32, device=dev))  # fmt: skip
+    out = Sequences(empty_matrices(groups, beams, steps, torch.int32), empty_matrix(groups, beams, torch.int32))
     if groups:
-        launch(dev.index, "leat_beam_sequences", _lib.lib.leat_beam_sequences, tokens.data_ptr(), parents.data_ptr(), steps, groups, beams,
-               -1 if end_id is None else end_id, out.tokens.data_ptr(), out.lengths.data_ptr())  # fmt: skip
+        code = _lib.lib.leat_beam_sequences(tokens.data_ptr(), parents.data_ptr(), steps, groups, beams, -1 if end_id is None else end_id,
+                                            out.tokens.data_ptr(), out.lengths.data_ptr(), raw_stream(dev.index))  # fmt: skip
+        if code != _lib.OK:
+            _lib.check(code, "leat_beam_sequences")
     return out
 
 

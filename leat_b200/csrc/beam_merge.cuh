@@ -125,9 +125,9 @@ struct Beam {
 __device__ __forceinline__ double score_of(const Beam& b, float x) {
   return b.base + ((double)fminf(x, largest_float()) - (double)b.max);
 }
-// Ranks to within 2^-21 of themselves and of the beam's reach, scale * (|base| + 8), enough to leave most
-// logits out: 2^-24 for the base's, the scale's and the difference's rounding and for the sum's and the
-// product's, and 2^-19 for the base's own error.  A beam that is not live has a NaN for its base.
+// Ranks to within 2^-17 of themselves and of the beam's reach, scale * (|base| + 8), enough to leave most
+// logits out: 2^-24 each for the rounding of the base, the difference, the sum and the product, 2^-19 for
+// the base's own error, 2^-17 for the scale's.  A beam that is not live has a NaN for its base.
 struct __align__(16) Near {
   float base, max, scale, pad;
 };
@@ -195,7 +195,7 @@ __device__ __forceinline__ void exact_is_known() {
 //   beam(u)            the unit's beam
 //   peek(u, k)         the largest logit of the lane's node
 //   token(u, k)        its first token
-//   each(u, k, visit)  calls visit(logit, token) for what the node puts on the list (SELF: the node
+//   each(u, k, visit)  calls visit(logit, token, number) for what the node puts on the list (SELF: the node
 //                      itself; else its logits)
 // Units of beams that are not live hold nothing, but may be read.  There are no branches where a unit is
 // looked at: the block does little else than wait for loads, and a branch between two would have the
@@ -213,7 +213,7 @@ __device__ __noinline__ void one_by_one(Level& L, int which, int units, int want
 #pragma unroll 1
     for (int u = warp; u < units; u += WARPS) {
       const int k = unit.beam(u);
-      unit.each(u, k, [&](float x, int token) {
+      unit.each(u, k, [&](float x, int token, int) {
         if (near_rank(L.near[k], x) == 0u) return;
         const Node v = node_of(L.beams, Pick{x, token, k});
         if ((last.beam < 0 || goes_before(last, v)) && (mine.beam < 0 || goes_before(v, mine))) mine = v;
@@ -326,27 +326,44 @@ __device__ __forceinline__ int best_nodes(Level& L, int which, int units, int wa
   unsigned bound = 1u;
   if (at_least > 0u) {
     const float b = unord32(at_least);
-    if (b > neg_inf()) bound = ord32(b - 9.5367431640625e-07f * (fabsf(b) + L.reach) + 0.0f);  // 2^-20: both sides' errors
+    if (b > neg_inf()) bound = ord32(b - 3.0517578125e-05f * (fabsf(b) + L.reach) + 0.0f);  // 2^-15: both sides' errors
   }
   auto collect = [&](int base, const Batch& b) {
+    unsigned hits[AHEAD];
+    int n = 0;
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      const unsigned hits = __ballot_sync(FULL, b.bits[a] >= bound);
-      if (hits == 0u) continue;
-      const int u = base + a * WARPS, k = b.k[a];
-      if (Unit::SELF) {
-        int at = 0;
-        if (lane == 0) at = atomicAdd(&L.found[which], __popc(hits));
-        at = __shfl_sync(FULL, at, 0) + __popc(hits & ((1u << lane) - 1u));
-        if ((hits >> lane & 1u) && at < BM_LIST) L.list[which][at] = Pick{b.x[a], unit.token(u, k), k};
-      } else if (hits >> lane & 1u) {
-        const Near near = L.near[k];
-        unit.each(u, k, [&](float x, int token) {
-          if (near_rank(near, x) >= bound) {
-            const int at = atomicAdd(&L.found[which], 1);
+      hits[a] = __ballot_sync(FULL, b.bits[a] >= bound);
+      n += __popc(hits[a]);
+    }
+    if (n == 0) return;
+    if (Unit::SELF) {
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&L.found[which], n);
+      at = __shfl_sync(FULL, at, 0);
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        const int mine = at + __popc(hits[a] & ((1u << lane) - 1u));
+        if ((hits[a] >> lane & 1u) && mine < BM_LIST) L.list[which][mine] = Pick{b.x[a], unit.token(base + a * WARPS, b.k[a]), b.k[a]};
+        at += __popc(hits[a]);
+      }
+    } else {
+#pragma unroll 1
+      for (int a = 0; a < AHEAD; ++a) {
+        const int u = base + a * WARPS;
+        if (u >= units || hits[a] == 0u) continue;
+        if (hits[a] >> lane & 1u) {
+          const int k = unit.beam(u);
+          const Near near = L.near[k];
+          unsigned some = 0u;
+          unit.each(u, k, [&](float x, int, int q) { some |= (near_rank(near, x) >= bound ? 1u : 0u) << q; });
+          int at = atomicAdd(&L.found[which], __popc(some));
+          unit.each(u, k, [&](float x, int token, int q) {
+            if (!(some >> q & 1u)) return;
             if (at < BM_LIST) L.list[which][at] = Pick{x, token, k};
-          }
-        });
+            ++at;
+          });
+        }
       }
     }
   };
@@ -390,7 +407,7 @@ struct TileUnit {
   __device__ __forceinline__ int token(int u, int k) const { return place(u, k) * tile_logits(FMT != 0); }
   template <typename Visit>
   __device__ __forceinline__ void each(int u, int k, Visit&& visit) const {
-    visit(peek(u, k), token(u, k));
+    visit(peek(u, k), token(u, k), 0);
   }
 };
 // the 32 chunks of a tile: of all the group's tiles, or of those on the list
@@ -411,7 +428,7 @@ struct ChunkUnit {
   }
   template <typename Visit>
   __device__ __forceinline__ void each(int u, int k, Visit&& visit) const {
-    visit(peek(u, k), token(u, k));
+    visit(peek(u, k), token(u, k), 0);
   }
 };
 // the 32 vectors of a chunk on the list, which put their logits on the next
@@ -460,7 +477,7 @@ struct VectorUnit {
     load(u, k, w);
     const int first = token(u, k);
 #pragma unroll
-    for (int q = 0; q < PER; ++q) visit(held<FMT>(w, q), first + q);
+    for (int q = 0; q < PER; ++q) visit(held<FMT>(w, q), first + q, q);
   }
 };
 
@@ -487,6 +504,13 @@ __device__ __forceinline__ int best_of_rows(Level& L, const TileParams& T, int r
 // the length penalty: ((5 + length) / 6)^alpha
 __device__ __noinline__ double length_divisor(int length, float alpha) {
   return pow((5.0 + (double)max(length, 0)) / 6.0, (double)alpha);
+}
+
+// its reciprocal, to within 2^-17 (for 32-bit lengths and |alpha| up to 4; 2^-20 for lengths up to 10^5 and 1)
+__device__ __forceinline__ float near_scale(int length, float alpha) {
+  float log2_l;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(log2_l) : "f"((5.0f + (float)max(length, 0)) * (1.0f / 6.0f)));
+  return ex2(-alpha * log2_l);
 }
 
 // a rank as ordered bits, so that candidates compare as whole numbers
@@ -547,7 +571,7 @@ __global__ void __launch_bounds__(THREADS + BM_EXACT) beam_merge_kernel(const Me
     }
     if (lane == 0) {
       const float base = score - (float)sum.log;
-      const float scale = P.length_penalty == 0.0f ? 1.0f : (float)(1.0 / length_divisor(length, P.length_penalty));
+      const float scale = P.length_penalty == 0.0f ? 1.0f : near_scale(length, P.length_penalty);
       const bool any = sum.max > neg_inf();
       L.near[k] = Near{any ? base : quiet_nan(), sum.max, scale, 0.0f};
       if (any) atomicMax(reinterpret_cast<int*>(&L.reach), __float_as_int(scale * (fabsf(base) + 8.0f)));

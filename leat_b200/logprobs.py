@@ -44,31 +44,36 @@ def _scratch_bytes(rows: int, vocab: int, width: int) -> int:
     size = _lib.lib.leat_beam_workspace_bytes(rows, vocab, width)
     if size == 0:
         raise ValueError(f"({rows}, {vocab}) logits are beyond the kernels' sizes")
-    return size
+    return size + 256
 
 
-def scratch(rows: int, vocab: int, width: int, device) -> tuple[torch.Tensor, int, int]:
-    """A call's workspace: the tensor that holds it, its 256-byte aligned address and its size.  It is
-    the call's own (the caching allocator keeps it for the current stream), so calls on several
-    streams or in several graphs share nothing."""
+# A call's time on the host is most of what a small one takes, so two of torch's inner entry points are
+# used where they are there: the current stream's handle without a Stream object around it (0.1 us for
+# 3.2), and memory of the current device without the keyword arguments' parsing (0.8 us for 1.8).
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_empty_strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+if _empty_strided is None:
+
+    def _empty_strided(size, stride, dtype):
+        return torch.empty_strided(size, stride, dtype=dtype, device="cuda")
+
+
+def empty_matrix(rows: int, columns: int, dtype: torch.dtype) -> torch.Tensor:
+    """(rows, columns) of the current device's memory, uninitialised."""
+    return _empty_strided((rows, columns), (columns, 1), dtype)
+
+
+def empty_matrices(count: int, rows: int, columns: int, dtype: torch.dtype) -> torch.Tensor:
+    return _empty_strided((count, rows, columns), (rows * columns, columns, 1), dtype)
+
+
+def scratch(rows: int, vocab: int, width: int) -> tuple[torch.Tensor, int, int]:
+    """A call's workspace on the current device: the tensor that holds it, its 256-byte aligned address and
+    its size.  It is the call's own (the caching allocator keeps it for the current stream), so calls on
+    several streams or in several graphs share nothing."""
     size = _scratch_bytes(rows, vocab, width)
-    held = torch.empty(size + 256, dtype=torch.uint8, device=device)
-    return held, (held.data_ptr() + 255) & ~255, size
-
-
-# the current stream's handle without a Stream object around it (3 us of a 15 us call), where torch has it
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
-def launch(index: int, what: str, call, *args) -> None:
-    """call(*args, stream) on CUDA device `index` and its current stream."""
-    if torch.cuda.current_device() == index:
-        code = call(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            code = call(*args, _raw_stream(index))
-    if code != _lib.OK:
-        _lib.check(code, what)
+    held = _empty_strided((size,), (1,), torch.uint8)
+    return held, (held.data_ptr() + 255) & ~255, size - 256
 
 
 def token_logprobs(logits, ids=None, top: int = 0) -> TokenLogprobs:
@@ -79,8 +84,11 @@ def token_logprobs(logits, ids=None, top: int = 0) -> TokenLogprobs:
     A NaN logit counts as -inf.  Ids outside the vocabulary (a -1 of padding) and tokens of logit -inf
     have log-probability -inf, as does everything in a row without a logit above -inf."""
     logits = rows_of_logits(logits)
-    rows, vocab = logits.shape
     dev = logits.device
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return token_logprobs(logits, ids, top)
+    rows, vocab = logits.shape
     if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= MAX_TOP:
         raise ValueError(f"top must be an integer from 0 to {MAX_TOP}")
     given = 0
@@ -95,16 +103,18 @@ def token_logprobs(logits, ids=None, top: int = 0) -> TokenLogprobs:
             ids = ids.clamp(-1, vocab).to(torch.int32)
         if not ids.is_contiguous():
             ids = ids.contiguous()
-    out = TokenLogprobs(torch.empty(rows, given, dtype=torch.float32, device=dev) if ids is not None else None)
+    out = TokenLogprobs(None if ids is None else empty_matrix(rows, given, torch.float32))
     if top:
-        out.top_logprobs = torch.empty(rows, top, dtype=torch.float32, device=dev)
-        out.top_ids = torch.empty(rows, top, dtype=torch.int32, device=dev)
+        out.top_logprobs = empty_matrix(rows, top, torch.float32)
+        out.top_ids = empty_matrix(rows, top, torch.int32)
     if rows == 0 or given + top == 0:
         return out
-    held, at, size = scratch(rows, vocab, top, dev)
+    held, at, size = scratch(rows, vocab, top)
     a = _lib.LogprobArgs(
         logits.data_ptr(), rows, vocab, logits.stride(0), FORMATS[logits.dtype], given, top, ids.data_ptr() if given else None,
         out.logprobs.data_ptr() if given else None, out.top_logprobs.data_ptr() if top else None,
         out.top_ids.data_ptr() if top else None, at, size)  # fmt: skip
-    launch(dev.index, "leat_token_logprobs", _lib.lib.leat_token_logprobs, a)
+    code = _lib.lib.leat_token_logprobs(a, raw_stream(dev.index))
+    if code != _lib.OK:
+        _lib.check(code, "leat_token_logprobs")
     return out
