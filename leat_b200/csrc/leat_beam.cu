@@ -171,7 +171,9 @@ int leat_reorder_states(const leat_state* states, int32_t count, const int32_t* 
   memset(&P, 0, sizeof(P));
   P.parents = parents; P.slots = slots; P.start = start; P.end = end;
   P.start_all = start_all; P.end_all = end_all; P.beams = beams;
-  const size_t shared = (size_t)beams * RO_THREADS * 16;
+  const bool twice = beams <= 16;
+  const int span = RO_THREADS * column_bytes(twice);  // bytes of a row that a block takes at a time
+  const size_t shared = (size_t)beams * span;
   // one launch per width of the widest loads that a tensor allows (16, 8, 4, 2, 1 bytes) and 64 of its kind
   for (int unit = 16; unit >= 1; unit /= 2) {
     int next = 0;
@@ -191,17 +193,20 @@ int leat_reorder_states(const leat_state* states, int32_t count, const int32_t* 
         int64_t places = s.places;
         if (!start && !end) places = (end_all < places ? end_all : places) - (start_all > 0 ? start_all : 0);
         if (places < 0) places = 0;
-        const long long here = (places * s.place_bytes + RO_THREADS * 16 - 1) / (RO_THREADS * 16) * s.outer;
+        const long long here = (places * s.place_bytes + span - 1) / span * s.outer;
         if (here > chunks) chunks = here;
       }
       if (n == 0 || chunks == 0) continue;
-      // about 32 blocks per SM of 148 in all: many short blocks balance rows that move and rows that stay
-      long long x = (148 * 32 + (long long)groups * n - 1) / ((long long)groups * n);
+      // many short blocks: they balance groups whose rows move and groups whose rows stay
+      long long x = (148 * 128 + (long long)groups * n - 1) / ((long long)groups * n);
       if (x > chunks) x = chunks;
       const dim3 grid((unsigned)x, (unsigned)groups, (unsigned)n);
-      auto kernel = unit == 16 ? reorder_kernel<16> : unit == 8 ? reorder_kernel<8> : unit == 4 ? reorder_kernel<4>
-                    : unit == 2 ? reorder_kernel<2> : reorder_kernel<1>;
-      if (shared > 48 * 1024 &&
+      auto kernel = twice ? (unit == 16 ? reorder_kernel<16, true> : unit == 8 ? reorder_kernel<8, true> : unit == 4 ? reorder_kernel<4, true>
+                             : unit == 2 ? reorder_kernel<2, true> : reorder_kernel<1, true>)
+                          : (unit == 16 ? reorder_kernel<16, false> : unit == 8 ? reorder_kernel<8, false> : unit == 4 ? reorder_kernel<4, false>
+                             : unit == 2 ? reorder_kernel<2, false> : reorder_kernel<1, false>);
+      if (shared > 40 * 1024 &&  // (beside what the kernel declares, 48 KB without asking)
+          
           cuda_failed(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared), "cudaFuncSetAttribute"))
         return LEAT_E_CUDA;
       if (cuda_failed(launch_dependent(kernel, grid, dim3(RO_THREADS), shared, stream, P), "reorder_kernel launch"))

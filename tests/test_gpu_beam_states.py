@@ -48,7 +48,7 @@ def _plain_rows(groups, beams):
     return np.arange(groups * beams).reshape(groups, beams)
 
 
-@pytest.mark.parametrize("beams", [1, 2, 3, 5, 8, 17, 32, 33, 64])
+@pytest.mark.parametrize("beams", [1, 2, 3, 5, 8, 12, 16, 17, 23, 24, 32, 33, 64])
 def test_parents_of_every_kind(device, beams):
     import torch
 

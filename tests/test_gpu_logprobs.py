@@ -74,6 +74,28 @@ def test_masks_ties_and_infinities(device, kind, vocab):
     _check(got, logits.double().cpu().numpy(), ids.numpy(), 64)
 
 
+def test_more_rows_than_a_grid_is_high(device):
+    import torch
+
+    from leat_b200.logprobs import token_logprobs
+
+    rows = 70001
+    logits = torch.randn((rows, 40), generator=torch.Generator().manual_seed(5)).to(device)
+    ids = torch.randint(0, 40, (rows, 1), generator=torch.Generator().manual_seed(6), dtype=torch.int32)
+    _check(token_logprobs(logits, ids.to(device), 3), logits.double().cpu().numpy(), ids.numpy(), 3)
+
+
+def test_more_given_ids_than_a_warp(device):
+    import torch
+
+    from leat_b200.logprobs import token_logprobs
+
+    logits = torch.randn((5, 700), generator=torch.Generator().manual_seed(7)).to(device)
+    ids = torch.randint(-2, 702, (5, 75), generator=torch.Generator().manual_seed(8), dtype=torch.int32)
+    for top in (0, 2, 30):
+        _check(token_logprobs(logits, ids.to(device), top), logits.double().cpu().numpy(), ids.numpy(), top)
+
+
 def test_ids_beyond_32_bits_are_outside(device):
     import torch
 
