@@ -187,8 +187,9 @@ def reorder_states(states, parents: torch.Tensor, *, slots: torch.Tensor | None 
     """Makes per-beam states follow their beams, in place: in every tensor of `states`, the row of beam k
     of group g takes what the row of beam parents[g, k] held.  Rows that keep their place are not touched.
 
-    states: a tensor or a list of them, of any type, rows first; row g * K + k belongs to beam k of group
-    g, or row slots[g, k] where `slots` (G, K) int32 is given (cache slots; all different).  parents (G, K)
+    states: a tensor or a list of them, of any type, rows first, no two of the same memory; row g * K + k
+    belongs to beam k of group g, or row slots[g, k] where `slots` (G, K) int32 is given (cache slots; all
+    different: the rows of a slot that two beams share are either's).  parents (G, K)
     int32, K up to 64, as beam_select returns them.
 
     `dim`: the dimension that counts positions, the same in every tensor (a cache (rows, heads,
@@ -218,6 +219,7 @@ def reorder_states(states, parents: torch.Tensor, *, slots: torch.Tensor | None 
     end_at, end_all, keep_end = _range_end(0x7FFFFFFF if length is None else length, groups, dev, "length")
     # a search's caches are mostly alike: what one comes to holds for the next of its shape and strides
     described: list[bytes] = []
+    where = []
     shape = dtype = stride = None
     plain = False  # the last was contiguous: the next is alike if it is, too
     for t in states:
@@ -237,9 +239,13 @@ def reorder_states(states, parents: torch.Tensor, *, slots: torch.Tensor | None 
                 raise ValueError("the rows of a state must not overlap")
             shape, dtype, stride, plain = t.shape, t.dtype, t.stride(), t.is_contiguous()
             rest = pack(STATE_REST, *like, 0)
-        described.append(pack("P", t.data_ptr()) + rest)
+        at = t.data_ptr()
+        where.append(at)
+        described.append(pack("P", at) + rest)
     if not described or groups == 0:
         return
+    if len(set(where)) != len(where):
+        raise ValueError("a state may only be given once: it would be reordered twice, at the same time")
     code = _lib.lib.leat_reorder_states(b"".join(described), len(described), parents.data_ptr(), None if slots is None else slots.data_ptr(),
                                         groups, beams, start_at, start_all, end_at, end_all, raw_stream(index))  # fmt: skip
     if code != _lib.OK:

@@ -125,9 +125,10 @@ struct Beam {
 __device__ __forceinline__ double score_of(const Beam& b, float x) {
   return b.base + ((double)fminf(x, largest_float()) - (double)b.max);
 }
-// Ranks to within 2^-17 of themselves and of the beam's reach, scale * (|base| + 8), enough to leave most
-// logits out: 2^-24 each for the rounding of the base, the difference, the sum and the product, 2^-19 for
-// the base's own error, 2^-17 for the scale's.  A beam that is not live has a NaN for its base.
+// Ranks to within a margin of themselves and of the beam's reach, scale * (|base| + 8), enough to leave
+// most logits out: 2^-24 each for the rounding of the base, the difference, the sum and the product and
+// 2^-19 of 1 for the base's own error (so 2^-20 of the reach in all), and with a length penalty 2^-17
+// for the scale's.  A beam that is not live has a NaN for its base.
 struct __align__(16) Near {
   float base, max, scale, pad;
 };
@@ -164,7 +165,8 @@ struct Level {
   float stage[STAGE];  // the tiles' maxima, if they fit
   Beam beams[BM_MAX_BEAMS];
   Near near[BM_MAX_BEAMS];
-  float reach;  // largest scale * (|base| + 8) of the live beams
+  float reach;   // largest scale * (|base| + 8) of the live beams
+  float margin;  // how far two near ranks may be off together, relative to theirs and the reach
   Pick list[2][BM_LIST];
   __align__(16) unsigned part_best[BM_PARTS];
   int found[2];  // (one per list: a slow thread may still read one while the next level clears the other)
@@ -242,6 +244,50 @@ __device__ __noinline__ void one_by_one(Level& L, int which, int units, int want
   }
 }
 
+// what is on a list, as units (each lane's of its own beam)
+template <typename Level>
+struct ListUnit {
+  Level& L;
+  int which, n;
+  __device__ __forceinline__ int at(int u) const { return min(u * 32 + (int)(threadIdx.x & 31), n - 1); }
+  __device__ __forceinline__ int beam(int u) const { return L.list[which][at(u)].beam; }
+  __device__ __forceinline__ float peek(int u, int) const { return u * 32 + (int)(threadIdx.x & 31) < n ? L.list[which][at(u)].x : neg_inf(); }
+};
+// A bound that between `want` and `most` of the units' nodes reach, by bisection with counts over the
+// block between lo, which enough reach, and hi, which none does; 0 if there is none.
+template <typename Level, typename Unit>
+__device__ __noinline__ unsigned tighter_bound(Level& L, int units, int want, int most, unsigned lo, unsigned hi, Unit unit) {
+  constexpr int WARPS = Level::THREADS / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  bool fits = false;
+  level_sync<Level>();
+#pragma unroll 1
+  for (int round = 0; hi - lo > 1u && !fits; ++round) {
+    const unsigned mid = lo + (hi - lo) / 2u;
+    int n = 0;
+#pragma unroll 4
+    for (int u = warp; u < units; u += WARPS) {
+      const int k = unit.beam(u);
+      n += near_rank(L.near[k], unit.peek(u, k)) >= mid ? 1 : 0;
+    }
+    n = __reduce_add_sync(FULL, n);
+    int* counts = reinterpret_cast<int*>(L.part_best) + (round & 1) * WARPS;  // (in turn: one barrier a round)
+    if (lane == 0) counts[warp] = n;
+    level_sync<Level>();
+    n = 0;
+#pragma unroll 1
+    for (int w = 0; w < WARPS; ++w) n += counts[w];
+    if (n >= want) {
+      lo = mid;
+      fits = n <= most;
+    } else {
+      hi = mid;
+    }
+  }
+  level_sync<Level>();
+  return fits ? lo : 0u;
+}
+
 // The `want` best nodes, and possibly a few more, into L.list[which], in no order; returns how many.
 // Every part of the block takes its best near rank, and each warp finds a bound that at least `want` of
 // the parts reach; what is not clearly below it goes on the list.  If that is more than the list holds
@@ -277,7 +323,7 @@ __device__ __forceinline__ int best_nodes(Level& L, int which, int units, int wa
     look(base, b);
     best = max(best, max(max(b.bits[0], b.bits[1]), max(b.bits[2], b.bits[3])));
   }
-  unsigned at_least;  // 0: fewer parts than wanted have any
+  unsigned at_least, top;  // 0: fewer parts than wanted have any; and what no node reaches
   if (few) {
     constexpr int LANES = THREADS / 32;
 #pragma unroll
@@ -294,6 +340,7 @@ __device__ __forceinline__ int best_nodes(Level& L, int which, int units, int wa
       before += (o.x > mine ? 1 : 0) + (o.y > mine ? 1 : 0) + (o.z > mine ? 1 : 0) + (o.w > mine ? 1 : 0);
     }
     at_least = __shfl_sync(FULL, mine, __ffs(__ballot_sync(FULL, before == want - 1)) - 1) & ~31u;
+    top = (__reduce_max_sync(FULL, mine) | 31u) + 1u;
   } else {
     constexpr int LANES = THREADS / BM_PARTS;
 #pragma unroll
@@ -309,7 +356,7 @@ __device__ __forceinline__ int best_nodes(Level& L, int which, int units, int wa
       lo = min(lo, v[j]);
     }
     lo = __reduce_min_sync(FULL, want <= 32 ? hi : lo);  // (each lane has one at least as large as its largest)
-    hi = __reduce_max_sync(FULL, hi) + 1u;
+    hi = top = __reduce_max_sync(FULL, hi) + 1u;
     const int enough = want + want / 2 + 4;
 #pragma unroll 1
     while (hi - lo > 1u) {
@@ -323,11 +370,12 @@ __device__ __forceinline__ int best_nodes(Level& L, int which, int units, int wa
     }
     at_least = lo;
   }
-  unsigned bound = 1u;
-  if (at_least > 0u) {
-    const float b = unord32(at_least);
-    if (b > neg_inf()) bound = ord32(b - 3.0517578125e-05f * (fabsf(b) + L.reach) + 0.0f);  // 2^-15: both sides' errors
-  }
+  // (0: fewer parts than wanted have any, and all nodes are taken)
+  auto with_margin = [&](unsigned bits) {
+    const float b = unord32(bits);
+    return bits > 0u && b > neg_inf() ? ord32(b - L.margin * (fabsf(b) + L.reach) + 0.0f) : 1u;
+  };
+  unsigned bound = with_margin(at_least);
   auto collect = [&](int base, const Batch& b) {
     unsigned hits[AHEAD];
     int n = 0;
@@ -367,15 +415,37 @@ __device__ __forceinline__ int best_nodes(Level& L, int which, int units, int wa
       }
     }
   };
-  collect(warp, first);
+  auto collect_all = [&]() {
+    collect(warp, first);
 #pragma unroll 1
-  for (int base = warp + WARPS * AHEAD; base < units; base += WARPS * AHEAD) {
-    Batch b;
-    look(base, b);
-    collect(base, b);
-  }
-  level_sync<Level>();
-  const int found = L.found[which];
+    for (int base = warp + WARPS * AHEAD; base < units; base += WARPS * AHEAD) {
+      Batch b;
+      look(base, b);
+      collect(base, b);
+    }
+    level_sync<Level>();
+    return L.found[which];
+  };
+  int found = collect_all();
+  // Where the best lie close together (masked rows, ramps), one part's best says little about the
+  // others' and the bound lets too many through: a node on the list costs the next level a unit.  What
+  // has got onto the list, all or some of it, gives a better one; where that leads nowhere, the nodes
+  // themselves do; and where many ranks are equal, none does.
+  const int loose = Unit::SELF ? 3 * want + 64 : BM_LIST;
+  auto again = [&](unsigned tight) {
+    const unsigned next = tight > 0u ? with_margin(tight) : 0u;
+    if (next <= bound) return false;
+    bound = next;
+    if (tid == 0) L.found[which] = 0;
+    level_sync<Level>();
+    found = collect_all();
+    return true;
+  };
+#pragma unroll 1
+  for (int tries = 0; found > loose && tries < 3; ++tries)
+    if (!again(tighter_bound(L, (min(found, BM_LIST) + 31) / 32, want, 2 * want, bound, top, ListUnit<Level>{L, which, min(found, BM_LIST)}))) break;
+  if (found <= BM_LIST) return found;
+  again(tighter_bound(L, units, want, Unit::SELF ? BM_LIST : BM_LIST / 8, bound, top, unit));
   if (found <= BM_LIST) return found;
   wait_for_exact<Level>(known);
   one_by_one(L, which, units, want, unit);
@@ -534,6 +604,7 @@ __global__ void __launch_bounds__(THREADS + BM_EXACT) beam_merge_kernel(const Me
   const int start = start_of(L, P.beams * tiles);
   if (tid == 0) {
     L.reach = 0.0f;
+    L.margin = P.length_penalty == 0.0f ? 1.9073486328125e-06f : 3.0517578125e-05f;  // 2^-19, 2^-15
     finished_n = 0;
   }
   __syncthreads();
@@ -667,6 +738,7 @@ __global__ void __launch_bounds__(THREADS + LP_EXACT) logprob_kernel(const Logpr
     if (lane == 0) {
       L.near[0] = Near{sum.max > neg_inf() ? -(float)sum.log : quiet_nan(), sum.max, 1.0f, 0.0f};
       L.reach = fabsf((float)sum.log) + 8.0f;
+      L.margin = 1.9073486328125e-06f;
     }
   }
   level_sync<RowLevel>();

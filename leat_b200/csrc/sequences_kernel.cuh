@@ -15,7 +15,7 @@
 
 namespace leat {
 
-constexpr int SQ_THREADS = 512;
+constexpr int SQ_THREADS = 256;
 constexpr int SQ_MAX_BEAMS = 64;
 constexpr int SQ_MAX_BLOCKS = 8;       // of a cluster
 constexpr int SQ_SHARED = 96 * 1024;   // nine bytes per step and beam: parent, token, path
@@ -44,7 +44,7 @@ __device__ __forceinline__ void cluster_publish(int warp) {
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
-__global__ void __launch_bounds__(SQ_THREADS, 3) sequences_kernel(const SequenceParams P) {
+__global__ void __launch_bounds__(SQ_THREADS, 6) sequences_kernel(const SequenceParams P) {
   namespace cg = cooperative_groups;
   extern __shared__ __align__(16) unsigned char dynamic[];
   __shared__ unsigned char run_map[2][SQ_THREADS];  // (runs, beams), a round's and the next's

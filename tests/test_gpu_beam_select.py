@@ -114,6 +114,41 @@ def test_many_large_logits_in_few_threads(device, kind):
     plain.check_selected(got, _numpy(logits), scores.cpu().numpy(), 64)
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("beams,vocab,allowed,width", [(8, 70000, 5, 8), (8, 70000, 5, 60), (1, 50000, 3, 8), (4, 40000, 1, 16), (24, 20000, 30, 48), (2, 33000, 9, 64)])
+def test_fewer_allowed_tokens_than_parts(device, kind, beams, vocab, allowed, width):
+    """All but a few tokens, side by side, at the type's lowest value: the best lie in one corner of the rows,
+    and where they are too few the lowest token ids among equals follow."""
+    import torch
+
+    from leat_b200.beam import beam_select
+
+    logits, scores = _inputs(2, beams, vocab, kind, 41, device)
+    kept = logits[:, 100:100 + allowed].clone()
+    logits[:] = torch.finfo(logits.dtype).min
+    logits[:, 100:100 + allowed] = kept
+    got = beam_select(logits, scores, width)
+    n = min(width, beams * allowed)
+    plain.check_selected(got, _numpy(logits), scores.cpu().numpy(), width)
+    assert bool(((got.tokens[:, :n] >= 100) & (got.tokens[:, :n] < 100 + allowed)).all())
+    if beams == 1:
+        assert got.tokens[:, n:].tolist() == [list(range(width - n))] * 2
+
+
+@pytest.mark.parametrize("vocab,width", [(60000, 8), (60000, 64), (300, 64)])
+def test_many_beams_of_one_ramp(device, vocab, width):
+    """Sorted rows that differ by their scores alone: every level's best lie side by side."""
+    import torch
+
+    from leat_b200.beam import beam_select
+
+    row = torch.linspace(30, 0, vocab, device=device)
+    scores = -torch.arange(12, device=device, dtype=torch.float32).reshape(2, 6) * 0.37
+    for logits in (row.expand(12, vocab).contiguous(), row.flip(0).expand(12, vocab).contiguous()):
+        got = beam_select(logits, scores, width)
+        plain.check_selected(got, _numpy(logits), scores.cpu().numpy(), width)
+
+
 def test_ascending_and_descending_logits(device):
     import torch
 

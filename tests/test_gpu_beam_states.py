@@ -209,7 +209,7 @@ def test_reorder_refusals(device):
         dict(dim=2, start=-1), dict(dim=2, length=-1), dict(dim=2, length=two), dict(dim=2, start=1.0), dict(dim=2, start=True),
         dict(states=t.transpose(2, 3), dim=2), dict(states=t[:, :, ::2], dim=2), dict(states=t[:1].expand(2, 3, 8, 4), dim=2),
         dict(states=t[:, :1].expand(2, 3, 8, 4), dim=2), dict(states=torch.zeros((), device=device)),
-        dict(states=t.clone().requires_grad_()), dict(states=t.transpose(1, 3)),
+        dict(states=[t, t]), dict(states=[t, t[:, :2]]), dict(states=t.clone().requires_grad_()), dict(states=t.transpose(1, 3)),
         dict(parents=torch.zeros((1, 65), dtype=torch.int32, device=device), states=torch.zeros((65, 4), device=device)),
     ]  # fmt: skip
     for more in bad:
