@@ -137,11 +137,10 @@ def _load() -> C.CDLL:
     lib.leat_shard_result.argtypes = [p, C.POINTER(SampleArgs), p]
     lib.leat_beam_workspace_bytes.restype = sz
     lib.leat_beam_workspace_bytes.argtypes = [i32, i32, i32]
-    lib.leat_beam_select.argtypes = [C.POINTER(BeamArgs), p]
-    lib.leat_reorder_states.argtypes = [p, i32,  # (a State array, or its bytes)
-                                          p, p, i32, i32, p, i32, p, i32, p]
+    lib.leat_beam_select.argtypes = [p, p]  # (a BeamArgs, by reference, or its bytes; so below)
+    lib.leat_reorder_states.argtypes = [p, i32, p, p, i32, i32, p, i32, p, i32, p]
     lib.leat_beam_sequences.argtypes = [p, p, i32, i32, i32, i32, p, p, p]
-    lib.leat_token_logprobs.argtypes = [C.POINTER(LogprobArgs), p]
+    lib.leat_token_logprobs.argtypes = [p, p]
     for name in EXPORTS:
         fn = getattr(lib, name)
         if name not in ("leat_sampler_workspace_bytes", "leat_beam_workspace_bytes", "leat_sampler_last_cuda_error", "leat_candidate_record_bytes",

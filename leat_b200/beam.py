@@ -14,10 +14,11 @@ from struct import pack
 import torch
 
 from leat_b200 import _lib
-from leat_b200.logprobs import FORMATS, empty_matrices, empty_matrix, raw_stream, rows_of_logits, scratch
+from leat_b200.logprobs import FORMATS, empty_strided, raw_stream, rows_of_logits, scratch
 
 MAX_BEAMS = 64
 MAX_WIDTH = 64
+SELECT_ARGS = "PiiiiqIiPPPf4xPPPPPPN"  # struct leat_beam_args
 STATE_REST = "qqqiiiI"  # struct leat_state behind its address, with the padding at its end
 
 
@@ -79,7 +80,7 @@ def beam_select(logits, scores: torch.Tensor, width: int | None = None, *, finis
         width = beams
     elif type(width) is not int or not 1 <= width <= MAX_WIDTH:
         raise ValueError(f"width must be an integer from 1 to {MAX_WIDTH}")
-    done_at = lengths_at = ended_at = new_lengths_at = None
+    done_at = lengths_at = ended_at = new_lengths_at = 0
     if end_id is not None:
         if type(end_id) is not int or not 0 <= end_id < vocab:
             raise ValueError("end_id must be a token of the vocabulary")
@@ -96,14 +97,15 @@ def beam_select(logits, scores: torch.Tensor, width: int | None = None, *, finis
     elif length_penalty != 0.0:
         raise ValueError("length_penalty needs the beams' lengths")
     if out is None:
-        out = Selected(empty_matrix(groups, width, torch.int32), empty_matrix(groups, width, torch.int32), empty_matrix(groups, width, torch.float32),
-                       None if end_id is None else empty_matrix(groups, width, torch.bool),
-                       None if lengths is None else empty_matrix(groups, width, torch.int32))  # fmt: skip
+        size, stride = (groups, width), (width, 1)
+        out = Selected(empty_strided(size, stride, torch.int32), empty_strided(size, stride, torch.int32), empty_strided(size, stride, torch.float32),
+                       None if end_id is None else empty_strided(size, stride, torch.bool),
+                       None if lengths is None else empty_strided(size, stride, torch.int32))  # fmt: skip
     else:
         wanted = [(out.tokens, torch.int32), (out.parents, torch.int32), (out.scores, torch.float32)]
         wanted += [(out.finished, torch.bool)] if end_id is not None else []
         wanted += [(out.lengths, torch.int32)] if lengths is not None else []
-        read = (scores.data_ptr(), lengths_at, done_at)
+        read = (scores.data_ptr(), lengths_at, done_at)  # (0 where there is none, as an empty tensor's)
         for t, dtype in wanted:
             if t is None or t.dtype != dtype or t.shape != (groups, width) or t.device != dev or not t.is_contiguous():
                 raise ValueError(f"out must hold contiguous ({groups}, {width}) tensors on {dev}, of the types of a Selected")
@@ -116,10 +118,9 @@ def beam_select(logits, scores: torch.Tensor, width: int | None = None, *, finis
     if lengths is not None:
         new_lengths_at = out.lengths.data_ptr()
     held, at, size = scratch(rows, vocab, width)
-    a = _lib.BeamArgs(
-        logits.data_ptr(), groups, beams, vocab, width, logits.stride(0), FORMATS[logits.dtype], -1 if end_id is None else end_id,
-        scores.data_ptr(), done_at, lengths_at, length_penalty, out.tokens.data_ptr(), out.parents.data_ptr(), out.scores.data_ptr(),
-        ended_at, new_lengths_at, at, size)  # fmt: skip
+    a = pack(SELECT_ARGS, logits.data_ptr(), groups, beams, vocab, width, logits.stride(0), FORMATS[logits.dtype], -1 if end_id is None else end_id,
+             scores.data_ptr(), done_at, lengths_at, length_penalty, out.tokens.data_ptr(), out.parents.data_ptr(), out.scores.data_ptr(),
+             ended_at, new_lengths_at, at, size)  # fmt: skip
     code = _lib.lib.leat_beam_select(a, raw_stream(dev.index))
     if code != _lib.OK:
         _lib.check(code, "leat_beam_select")
@@ -270,7 +271,8 @@ def beam_sequences(tokens: torch.Tensor, parents: torch.Tensor, end_id: int | No
         raise ValueError(f"there must be 1 to {MAX_BEAMS} beams")
     if end_id is not None and (isinstance(end_id, bool) or not isinstance(end_id, int) or not 0 <= end_id <= 0x7FFFFFFF):
         raise ValueError("end_id must be a token")
-    out = Sequences(empty_matrices(groups, beams, steps, torch.int32), empty_matrix(groups, beams, torch.int32))
+    shape = (groups, beams, steps)
+    out = Sequences(empty_strided(shape, (beams * steps, steps, 1), torch.int32), empty_strided((groups, beams), (beams, 1), torch.int32))
     if groups:
         code = _lib.lib.leat_beam_sequences(tokens.data_ptr(), parents.data_ptr(), steps, groups, beams, -1 if end_id is None else end_id,
                                             out.tokens.data_ptr(), out.lengths.data_ptr(), raw_stream(dev.index))  # fmt: skip

@@ -6,6 +6,7 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 from functools import lru_cache
+from struct import pack
 
 import torch
 
@@ -14,6 +15,7 @@ from leat_b200.sampler import device_tensor
 
 FORMATS = {torch.float32: 0, torch.bfloat16: _lib.FLAG_LOGITS_BF16, torch.float16: _lib.FLAG_LOGITS_F16}
 MAX_TOP = 64
+ARGS = "PiiqIii4xPPPPPN"  # struct leat_logprob_args
 
 
 @dataclass
@@ -51,20 +53,11 @@ def _scratch_bytes(rows: int, vocab: int, width: int) -> int:
 # used where they are there: the current stream's handle without a Stream object around it (0.1 us for
 # 3.2), and memory of the current device without the keyword arguments' parsing (0.8 us for 1.8).
 raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
-_empty_strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
-if _empty_strided is None:
+empty_strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+if empty_strided is None:
 
-    def _empty_strided(size, stride, dtype):
+    def empty_strided(size, stride, dtype):
         return torch.empty_strided(size, stride, dtype=dtype, device="cuda")
-
-
-def empty_matrix(rows: int, columns: int, dtype: torch.dtype) -> torch.Tensor:
-    """(rows, columns) of the current device's memory, uninitialised."""
-    return _empty_strided((rows, columns), (columns, 1), dtype)
-
-
-def empty_matrices(count: int, rows: int, columns: int, dtype: torch.dtype) -> torch.Tensor:
-    return _empty_strided((count, rows, columns), (rows * columns, columns, 1), dtype)
 
 
 def scratch(rows: int, vocab: int, width: int) -> tuple[torch.Tensor, int, int]:
@@ -72,7 +65,7 @@ def scratch(rows: int, vocab: int, width: int) -> tuple[torch.Tensor, int, int]:
     its size.  It is the call's own (the caching allocator keeps it for the current stream), so calls on
     several streams or in several graphs share nothing."""
     size = _scratch_bytes(rows, vocab, width)
-    held = _empty_strided((size,), (1,), torch.uint8)
+    held = empty_strided((size,), (1,), torch.uint8)
     return held, (held.data_ptr() + 255) & ~255, size - 256
 
 
@@ -103,17 +96,16 @@ def token_logprobs(logits, ids=None, top: int = 0) -> TokenLogprobs:
             ids = ids.clamp(-1, vocab).to(torch.int32)
         if not ids.is_contiguous():
             ids = ids.contiguous()
-    out = TokenLogprobs(None if ids is None else empty_matrix(rows, given, torch.float32))
+    out = TokenLogprobs(None if ids is None else empty_strided((rows, given), (given, 1), torch.float32))
     if top:
-        out.top_logprobs = empty_matrix(rows, top, torch.float32)
-        out.top_ids = empty_matrix(rows, top, torch.int32)
+        out.top_logprobs = empty_strided((rows, top), (top, 1), torch.float32)
+        out.top_ids = empty_strided((rows, top), (top, 1), torch.int32)
     if rows == 0 or given + top == 0:
         return out
     held, at, size = scratch(rows, vocab, top)
-    a = _lib.LogprobArgs(
-        logits.data_ptr(), rows, vocab, logits.stride(0), FORMATS[logits.dtype], given, top, ids.data_ptr() if given else None,
-        out.logprobs.data_ptr() if given else None, out.top_logprobs.data_ptr() if top else None,
-        out.top_ids.data_ptr() if top else None, at, size)  # fmt: skip
+    a = pack(ARGS, logits.data_ptr(), rows, vocab, logits.stride(0), FORMATS[logits.dtype], given, top, ids.data_ptr() if given else 0,
+             out.logprobs.data_ptr() if given else 0, out.top_logprobs.data_ptr() if top else 0, out.top_ids.data_ptr() if top else 0,
+             at, size)  # fmt: skip
     code = _lib.lib.leat_token_logprobs(a, raw_stream(dev.index))
     if code != _lib.OK:
         _lib.check(code, "leat_token_logprobs")

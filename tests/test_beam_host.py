@@ -22,7 +22,7 @@ def _select(**more):
              length_penalty=0.0, out_tokens=AT, out_parents=AT, out_scores=AT, out_finished=None, out_lengths=None, workspace=AT,
              workspace_bytes=0)  # fmt: skip
     a.update(more)
-    return _lib.lib.leat_beam_select(_lib.BeamArgs(**a), None)
+    return _lib.lib.leat_beam_select(C.byref(_lib.BeamArgs(**a)), None)
 
 
 def test_select_arguments():
@@ -53,7 +53,7 @@ def test_logprob_arguments():
         a = dict(logits=AT, rows=2, vocab=100, row_stride=100, flags=0, given=1, top=3, ids=AT, out_logprobs=AT, out_top_logprobs=AT,
                  out_top_ids=AT, workspace=AT, workspace_bytes=0)  # fmt: skip
         a.update(more)
-        return _lib.lib.leat_token_logprobs(_lib.LogprobArgs(**a), None)
+        return _lib.lib.leat_token_logprobs(C.byref(_lib.LogprobArgs(**a)), None)
 
     assert _lib.lib.leat_token_logprobs(None, None) == _lib.E_ARGUMENT
     for more in (dict(logits=None), dict(rows=-1), dict(vocab=0), dict(row_stride=50), dict(flags=12), dict(given=-1), dict(top=-1),
@@ -97,6 +97,20 @@ def test_struct_layouts_match_the_header(tmp_path, struct, name):
     subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-o", str(tmp_path / "layout"), str(tmp_path / "layout.c")], check=True)
     out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split()
     assert [int(v) for v in out] == [C.sizeof(struct)] + [getattr(struct, f).offset for f in fields]
+
+
+def test_packed_arguments_are_the_structs():
+    """The Python face packs a call's arguments itself; every field lies where the struct has it."""
+    import struct
+
+    from leat_b200 import beam, logprobs
+
+    for fmt, kind in ((beam.SELECT_ARGS, _lib.BeamArgs), (logprobs.ARGS, _lib.LogprobArgs), ("P" + beam.STATE_REST, _lib.State)):
+        assert struct.calcsize(fmt) == C.sizeof(kind)
+        values = [float(i + 1) if f[1] is C.c_float else i + 1 for i, f in enumerate(kind._fields_)]
+        extra = [0] if kind is _lib.State else []  # the padding at its end
+        got = kind.from_buffer_copy(struct.pack(fmt, *values, *extra))
+        assert [getattr(got, f) for f, _ in kind._fields_] == values
 
 
 def test_cpu_tensors_are_refused():
