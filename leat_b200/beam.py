@@ -360,7 +360,10 @@ class BeamSearch:
             reorder_states(states, out.parents, slots=slots, dim=dim, start=start, length=length)
         if history is not None:
             history.reorder(slots, out.parents)
-            history.append(slots, out.tokens)
+            tokens = out.tokens
+            if ends:  # what a finished beam goes on with is no token of its sequence
+                tokens = tokens.masked_fill(finished.gather(1, out.parents.long()), -1)
+            history.append(slots, tokens)
         self.steps += 1
         return out.tokens.clamp(min=0).reshape(-1, 1)
 

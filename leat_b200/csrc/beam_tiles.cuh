@@ -215,8 +215,9 @@ __global__ void __launch_bounds__(BT_THREADS, 7) beam_tile_kernel(const TilePara
   const bool empty = M == neg_inf(), plain = fabsf(M) < PLAIN_LIMIT;
   float s = (part[0] + part[1]) + (part[2] + part[3]);
   // once more, from the warp's maximum, where that did not do: the first chunk much below the others
-  // or all of them low, large values (differences first), a NaN or +inf
-  if (__any_sync(FULL, !have_e || !plain || !(s <= largest_float()))) {
+  // (the lanes' sums are still to be added up) or all of them low, large values (differences first), a
+  // NaN or +inf
+  if (__any_sync(FULL, !have_e || !plain || !(s <= 1e36f))) {
     e = ceilf(M * log2e());
     s = 0.0f;
     // (the words are taken as new here: widened logits kept for this from above would spill)

@@ -118,6 +118,26 @@ def test_step_keeps_history_itself_and_dead_beams_run_token_zero(device):
         search.step(logits, history=history)
 
 
+def test_a_finished_beam_adds_nothing_to_its_history(device):
+    import torch
+
+    from leat_b200.beam import BeamSearch
+    from leat_b200.history import SlotHistory
+
+    search = BeamSearch(1, 2, 4, end_id=3, device=device)
+    slots = torch.tensor([[0, 1]], dtype=torch.int32, device=device)
+    history = SlotHistory(2, 6, 20, device=device)
+    logits = torch.zeros((2, 20), device=device)
+    logits[:, 3], logits[:, 5] = 4.0, 3.9
+    for _ in range(3):
+        search.step(logits, slots=slots, history=history)
+    got = search.sequences()
+    for k in range(2):
+        length = int(got.lengths[0, k])
+        assert int(history.count[k]) == length and history.ids[k, :length].tolist() == got.tokens[0, k, :length].tolist()
+    assert int(got.lengths[0].min()) == 1 and bool(search.finished[0].any())
+
+
 @pytest.mark.parametrize("bad", [dict(groups=0), dict(beams=0), dict(beams=65), dict(max_steps=0)])
 def test_search_refusals(device, bad):
     from leat_b200.beam import BeamSearch

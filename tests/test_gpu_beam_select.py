@@ -177,6 +177,22 @@ def test_logits_near_the_largest_float(device, scale):
     assert abs(float(got.scores[1, 0]) + np.log(9000)) <= plain.LOG_SUM_ERROR + 10 * 2.0**-24
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("low,high", [(-62.0, 25.0), (-62.0, 22.5), (-62.0, 21.0), (-62.0, 20.0), (-40.0, 60.0), (-900.0, 10.0), (-1500.0, -1400.0), (30.0, -40.0)])
+def test_rows_that_begin_far_from_their_maximum(device, kind, low, high):
+    """The sums start from a row's first logits: the others may lie up to the exponentials' whole range above."""
+    import torch
+
+    from leat_b200.beam import beam_select
+
+    logits, scores = _inputs(2, 2, 9000, "float32", 23, device, scale=0.5)
+    logits += high
+    logits[:, :512] = low
+    logits = logits.to(getattr(torch, kind))
+    got = beam_select(logits, scores, 5)
+    plain.check_selected(got, _numpy(logits), scores.cpu().numpy(), 5)
+
+
 @pytest.mark.parametrize("alpha", [0.0, 0.6, 1.0, -0.5])
 @pytest.mark.parametrize("vocab", [40, 9001])
 def test_finished_dead_beams_and_lengths(device, alpha, vocab):
