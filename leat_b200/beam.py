@@ -9,6 +9,7 @@ scratch is its own, so every part can be captured into a CUDA graph."""
 from __future__ import annotations
 
 from dataclasses import dataclass
+from math import prod
 from struct import pack
 
 import torch
@@ -173,14 +174,16 @@ def _overlaps(row_stride: int, outer_stride: int, place_bytes: int, outer: int, 
     return not (rows_outside or rows_inside)
 
 
-def _range_end(x, groups: int, device, name: str):
-    """A bound of the places: (pointer or None, value for all groups, tensor to keep)."""
-    if isinstance(x, torch.Tensor):
-        x = _whole(x, torch.int32, (groups,), device, name)
-        return x.data_ptr(), 0, x
-    if isinstance(x, bool) or not isinstance(x, int) or x < 0:
+def _range_end(x, default: int, groups: int, device, name: str):
+    """A bound of the places: (pointer or None, value for all groups, what to keep until the launch)."""
+    if x is None:
+        return None, default, None
+    if type(x) is int and x >= 0:
+        return None, min(x, 0x7FFFFFFF), None
+    if not isinstance(x, torch.Tensor):
         raise ValueError(f"{name} must be a number of places, or a ({groups},) int32 tensor of them")
-    return None, min(x, 0x7FFFFFFF), None
+    x = _whole(x, torch.int32, (groups,), device, name)
+    return x.data_ptr(), 0, x
 
 
 def reorder_states(states, parents: torch.Tensor, *, slots: torch.Tensor | None = None, dim: int | None = None,
@@ -209,18 +212,24 @@ def reorder_states(states, parents: torch.Tensor, *, slots: torch.Tensor | None 
         with torch.cuda.device(dev):
             return reorder_states(states, parents, slots=slots, dim=dim, start=start, length=length)
     groups, beams = parents.shape
-    parents = _whole(parents, torch.int32, parents.shape, dev, "parents")
+    if parents.dtype != torch.int32:
+        raise ValueError("parents must be a (G, K) int32 CUDA tensor")
+    if not parents.is_contiguous():
+        parents = parents.contiguous()
     if not 1 <= beams <= MAX_BEAMS or groups > 65535:
         raise ValueError(f"parents must be (G, K) with K from 1 to {MAX_BEAMS} and G up to 65535")
+    slots_at = None
     if slots is not None:
         slots = _whole(slots, torch.int32, parents.shape, dev, "slots")
-    if dim is None and (length is not None or (start is not None and (isinstance(start, torch.Tensor) or start != 0))):
+        slots_at = slots.data_ptr()
+    start_at, start_all, end_at, end_all = None, 0, None, 0x7FFFFFFF
+    if dim is not None:
+        start_at, start_all, start = _range_end(start, 0, groups, dev, "start")
+        end_at, end_all, length = _range_end(length, 0x7FFFFFFF, groups, dev, "length")
+    elif length is not None or (start is not None and (isinstance(start, torch.Tensor) or start != 0)):
         raise ValueError("start and length count positions: say which dimension they are with dim")
-    start_at, start_all, keep_start = _range_end(0 if start is None else start, groups, dev, "start")
-    end_at, end_all, keep_end = _range_end(0x7FFFFFFF if length is None else length, groups, dev, "length")
     # a search's caches are mostly alike: what one comes to holds for the next of its shape and strides
     described: list[bytes] = []
-    where = []
     shape = dtype = stride = None
     plain = False  # the last was contiguous: the next is alike if it is, too
     for t in states:
@@ -235,23 +244,27 @@ def reorder_states(states, parents: torch.Tensor, *, slots: torch.Tensor | None 
                 raise ValueError("dim must be a dimension of every state, behind the rows'")
             if t.numel() == 0:
                 continue
-            like = _state(t, dim)
-            if _overlaps(*like):
-                raise ValueError("the rows of a state must not overlap")
-            shape, dtype, stride, plain = t.shape, t.dtype, t.stride(), t.is_contiguous()
-            rest = pack(STATE_REST, *like, 0)
-        at = t.data_ptr()
-        where.append(at)
-        described.append(pack("P", at) + rest)
-    if not described or groups == 0:
+            shape, dtype, plain = t.shape, t.dtype, t.is_contiguous()
+            if plain:
+                place, run = prod(shape[dim + 1:]) if dim is not None else prod(shape[1:]), shape[dim] if dim is not None else 1
+                outer, size = prod(shape[1:dim]) if dim is not None else 1, t.element_size()
+                rest = pack(STATE_REST, outer * run * place * size, run * place * size, place * size, outer, run, shape[0], 0)
+            else:
+                stride = t.stride()
+                like = _state(t, dim)
+                if _overlaps(*like):
+                    raise ValueError("the rows of a state must not overlap")
+                rest = pack(STATE_REST, *like, 0)
+        described.append(pack("P", t.data_ptr()) + rest)
+    count = len(described)
+    if count == 0 or groups == 0:
         return
-    if len(set(where)) != len(where):
+    if count > 1 and len({d[:8] for d in described}) != count:
         raise ValueError("a state may only be given once: it would be reordered twice, at the same time")
-    code = _lib.lib.leat_reorder_states(b"".join(described), len(described), parents.data_ptr(), None if slots is None else slots.data_ptr(),
-                                        groups, beams, start_at, start_all, end_at, end_all, raw_stream(index))  # fmt: skip
+    code = _lib.lib.leat_reorder_states(b"".join(described), count, parents.data_ptr(), slots_at, groups, beams,
+                                        start_at, start_all, end_at, end_all, raw_stream(index))  # fmt: skip
     if code != _lib.OK:
         _lib.check(code, "leat_reorder_states")
-    del keep_start, keep_end
 
 
 def beam_sequences(tokens: torch.Tensor, parents: torch.Tensor, end_id: int | None = None) -> Sequences:

@@ -244,6 +244,13 @@ __device__ __noinline__ void one_by_one(Level& L, int which, int units, int want
   }
 }
 
+// a near rank's bits less what two of them may be off; 1, which every node reaches, for 0
+template <typename Level>
+__device__ __forceinline__ unsigned with_margin(const Level& L, unsigned bits) {
+  const float b = unord32(bits);
+  return bits > 0u && b > neg_inf() ? ord32(b - L.margin * (fabsf(b) + L.reach) + 0.0f) : 1u;
+}
+
 // what is on a list, as units (each lane's of its own beam)
 template <typename Level>
 struct ListUnit {
@@ -288,6 +295,20 @@ __device__ __noinline__ unsigned tighter_bound(Level& L, int units, int want, in
   return fits ? lo : 0u;
 }
 
+// Where the best lie close together (masked rows, ramps), one part's best says little about the others' and
+// the bound lets too many through.  What has got onto the list, all or some of it, gives a better one;
+// where that leads nowhere, the nodes themselves do; and where many ranks are equal, none does (0).
+template <typename Level, typename Unit>
+__device__ __noinline__ unsigned next_bound(Level& L, int which, int units, int want, int found, int tries, unsigned bound, unsigned top, Unit unit) {
+  if (tries < 3) {
+    const int n = min(found, BM_LIST);
+    const unsigned next = with_margin(L, tighter_bound(L, (n + 31) / 32, want, 2 * want, bound, top, ListUnit<Level>{L, which, n}));
+    if (next > bound) return next;
+  }
+  if (found <= BM_LIST || tries > 3) return 0u;
+  return with_margin(L, tighter_bound(L, units, want, Unit::SELF ? BM_LIST : BM_LIST / 8, bound, top, unit));
+}
+
 // The `want` best nodes, and possibly a few more, into L.list[which], in no order; returns how many.
 // Every part of the block takes its best near rank, and each warp finds a bound that at least `want` of
 // the parts reach; what is not clearly below it goes on the list.  If that is more than the list holds
@@ -297,8 +318,9 @@ __device__ __forceinline__ int best_nodes(Level& L, int which, int units, int wa
   constexpr int THREADS = Level::THREADS, WARPS = THREADS / 32, AHEAD = 4, PER_LANE = BM_PARTS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (units == 0) return 0;
-  // 32 parts, one per lane of who compares them, where that makes enough; else BM_PARTS
-  const bool few = want <= BM_FEW && min(units, WARPS) * (32 / WARPS) >= want;
+  // 32 parts, one per lane of who compares them, where three times as many as wanted can have any;
+  // else BM_PARTS: a bound from too few parts lets too many nodes through
+  const bool few = min(units, WARPS) * (32 / WARPS) >= 3 * want;
   struct Batch {
     float x[AHEAD];
     int k[AHEAD];
@@ -370,12 +392,7 @@ __device__ __forceinline__ int best_nodes(Level& L, int which, int units, int wa
     }
     at_least = lo;
   }
-  // (0: fewer parts than wanted have any, and all nodes are taken)
-  auto with_margin = [&](unsigned bits) {
-    const float b = unord32(bits);
-    return bits > 0u && b > neg_inf() ? ord32(b - L.margin * (fabsf(b) + L.reach) + 0.0f) : 1u;
-  };
-  unsigned bound = with_margin(at_least);
+  unsigned bound = with_margin(L, at_least);  // (0: fewer parts than wanted have any, and all nodes are taken)
   auto collect = [&](int base, const Batch& b) {
     unsigned hits[AHEAD];
     int n = 0;
@@ -415,7 +432,11 @@ __device__ __forceinline__ int best_nodes(Level& L, int which, int units, int wa
       }
     }
   };
-  auto collect_all = [&]() {
+  // a node on the list costs the next level a unit; a logit on the last list costs next to nothing
+  const int loose = Unit::SELF ? 3 * want + 64 : BM_LIST;
+  int found, tries = 0;
+#pragma unroll 1
+  while (true) {
     collect(warp, first);
 #pragma unroll 1
     for (int base = warp + WARPS * AHEAD; base < units; base += WARPS * AHEAD) {
@@ -424,28 +445,14 @@ __device__ __forceinline__ int best_nodes(Level& L, int which, int units, int wa
       collect(base, b);
     }
     level_sync<Level>();
-    return L.found[which];
-  };
-  int found = collect_all();
-  // Where the best lie close together (masked rows, ramps), one part's best says little about the
-  // others' and the bound lets too many through: a node on the list costs the next level a unit.  What
-  // has got onto the list, all or some of it, gives a better one; where that leads nowhere, the nodes
-  // themselves do; and where many ranks are equal, none does.
-  const int loose = Unit::SELF ? 3 * want + 64 : BM_LIST;
-  auto again = [&](unsigned tight) {
-    const unsigned next = tight > 0u ? with_margin(tight) : 0u;
-    if (next <= bound) return false;
+    found = L.found[which];
+    if (found <= loose) return found;
+    const unsigned next = next_bound(L, which, units, want, found, tries++, bound, top, unit);
+    if (next <= bound) break;
     bound = next;
     if (tid == 0) L.found[which] = 0;
     level_sync<Level>();
-    found = collect_all();
-    return true;
-  };
-#pragma unroll 1
-  for (int tries = 0; found > loose && tries < 3; ++tries)
-    if (!again(tighter_bound(L, (min(found, BM_LIST) + 31) / 32, want, 2 * want, bound, top, ListUnit<Level>{L, which, min(found, BM_LIST)}))) break;
-  if (found <= BM_LIST) return found;
-  again(tighter_bound(L, units, want, Unit::SELF ? BM_LIST : BM_LIST / 8, bound, top, unit));
+  }
   if (found <= BM_LIST) return found;
   wait_for_exact<Level>(known);
   one_by_one(L, which, units, want, unit);

@@ -91,6 +91,17 @@ bool logits_fit(const void* logits, int rows, int vocab, long long row_stride, u
 
 int64_t lowest_bit(int64_t x) { return x & -x; }
 
+template <int UNIT>
+cudaError_t launch_reorder(const ReorderParams& P, dim3 grid, bool twice, cudaStream_t stream) {
+  const size_t shared = (size_t)P.beams * RO_THREADS * column_bytes(twice);
+  auto kernel = twice ? reorder_kernel<UNIT, true> : reorder_kernel<UNIT, false>;
+  if (shared > 40 * 1024) {  // (beside what the kernel declares, 48 KB without asking)
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+    if (e != cudaSuccess) return e;
+  }
+  return launch_dependent(kernel, grid, dim3(RO_THREADS), shared, stream, P);
+}
+
 }  // namespace
 
 extern "C" {
@@ -168,28 +179,23 @@ int leat_reorder_states(const leat_state* states, int32_t count, const int32_t* 
     if (s.outer > 1 && s.outer_stride < (int64_t)s.places * s.place_bytes) return LEAT_E_ARGUMENT;
   }
   ReorderParams P;
-  memset(&P, 0, sizeof(P));
   P.parents = parents; P.slots = slots; P.start = start; P.end = end;
   P.start_all = start_all; P.end_all = end_all; P.beams = beams;
   const bool twice = beams <= 16;
   const int span = RO_THREADS * column_bytes(twice);  // bytes of a row that a block takes at a time
-  const size_t shared = (size_t)beams * span;
   // one launch per width of the widest loads that a tensor allows (16, 8, 4, 2, 1 bytes) and 64 of its kind
   for (int unit = 16; unit >= 1; unit /= 2) {
     int next = 0;
     while (next < count) {
       int n = 0;
-      long long chunks = 0;
+      long long chunks = 0;  // of the tensor that has most to move
       for (; next < count && n < RO_MAX_STATES; ++next) {
         const leat_state& s = states[next];
         int64_t bits = (int64_t)(uintptr_t)s.data | s.place_bytes | 16;
         if (s.rows > 1) bits |= s.row_stride;
         if (s.outer > 1) bits |= s.outer_stride;
         if (lowest_bit(bits) != unit || s.rows == 0 || s.outer == 0 || s.places == 0) continue;
-        StateRows& to = P.states[n++];
-        to.data = static_cast<char*>(s.data);
-        to.row_stride = s.row_stride; to.outer_stride = s.outer_stride; to.place_bytes = s.place_bytes;
-        to.outer = s.outer; to.places = s.places; to.rows = s.rows; to.pad = 0;
+        P.states[n++] = StateRows{static_cast<char*>(s.data), s.row_stride, s.outer_stride, s.place_bytes, s.outer, s.places, s.rows, 0};
         int64_t places = s.places;
         if (!start && !end) places = (end_all < places ? end_all : places) - (start_all > 0 ? start_all : 0);
         if (places < 0) places = 0;
@@ -201,16 +207,10 @@ int leat_reorder_states(const leat_state* states, int32_t count, const int32_t* 
       long long x = (148 * 128 + (long long)groups * n - 1) / ((long long)groups * n);
       if (x > chunks) x = chunks;
       const dim3 grid((unsigned)x, (unsigned)groups, (unsigned)n);
-      auto kernel = twice ? (unit == 16 ? reorder_kernel<16, true> : unit == 8 ? reorder_kernel<8, true> : unit == 4 ? reorder_kernel<4, true>
-                             : unit == 2 ? reorder_kernel<2, true> : reorder_kernel<1, true>)
-                          : (unit == 16 ? reorder_kernel<16, false> : unit == 8 ? reorder_kernel<8, false> : unit == 4 ? reorder_kernel<4, false>
-                             : unit == 2 ? reorder_kernel<2, false> : reorder_kernel<1, false>);
-      if (shared > 40 * 1024 &&  // (beside what the kernel declares, 48 KB without asking)
-          
-          cuda_failed(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared), "cudaFuncSetAttribute"))
-        return LEAT_E_CUDA;
-      if (cuda_failed(launch_dependent(kernel, grid, dim3(RO_THREADS), shared, stream, P), "reorder_kernel launch"))
-        return LEAT_E_CUDA;
+      const cudaError_t e = unit == 16 ? launch_reorder<16>(P, grid, twice, stream) : unit == 8 ? launch_reorder<8>(P, grid, twice, stream)
+                            : unit == 4 ? launch_reorder<4>(P, grid, twice, stream) : unit == 2 ? launch_reorder<2>(P, grid, twice, stream)
+                            : launch_reorder<1>(P, grid, twice, stream);
+      if (cuda_failed(e, "reorder_kernel launch")) return LEAT_E_CUDA;
     }
   }
   return LEAT_OK;
