@@ -296,17 +296,43 @@ __device__ __noinline__ unsigned tighter_bound(Level& L, int units, int want, in
 }
 
 // Where the best lie close together (masked rows, ramps), one part's best says little about the others' and
-// the bound lets too many through.  What has got onto the list, all or some of it, gives a better one;
-// where that leads nowhere, the nodes themselves do; and where many ranks are equal, none does (0).
+// the bound lets too many nodes through.  What has got onto the list, all or some of it, gives a better one;
+// where that leads nowhere, the nodes themselves do; and where many ranks are equal, none does.  Returns how
+// many reach the best bound found.  (A function of its own, with nothing to go back to: in a loop with the
+// common path it made that slower by 1.5 us.)
 template <typename Level, typename Unit>
-__device__ __noinline__ unsigned next_bound(Level& L, int which, int units, int want, int found, int tries, unsigned bound, unsigned top, Unit unit) {
-  if (tries < 3) {
-    const int n = min(found, BM_LIST);
-    const unsigned next = with_margin(L, tighter_bound(L, (n + 31) / 32, want, 2 * want, bound, top, ListUnit<Level>{L, which, n}));
-    if (next > bound) return next;
+__device__ __noinline__ int fewer_nodes(Level& L, int which, int units, int want, int most, int found, unsigned bound, unsigned top, Unit unit) {
+  constexpr int WARPS = Level::THREADS / 32;
+#pragma unroll 1
+  for (int tries = 0; found > most && tries < 4; ++tries) {
+    unsigned next = 0u;
+    if (tries < 3) {
+      const int n = min(found, BM_LIST);
+      next = with_margin(L, tighter_bound(L, (n + 31) / 32, want, 2 * want, bound, top, ListUnit<Level>{L, which, n}));
+      if (next <= bound) tries = 3;
+    }
+    if (tries == 3) {
+      if (found <= BM_LIST) break;
+      next = with_margin(L, tighter_bound(L, units, want, Unit::SELF ? BM_LIST : BM_LIST / 8, bound, top, unit));
+      if (next <= bound) break;
+    }
+    bound = next;
+    if (threadIdx.x == 0) L.found[which] = 0;
+    level_sync<Level>();
+#pragma unroll 1
+    for (int u = threadIdx.x >> 5; u < units; u += WARPS) {
+      const int k = unit.beam(u);
+      if (near_rank(L.near[k], unit.peek(u, k)) < bound) continue;
+      unit.each(u, k, [&](float x, int token, int) {
+        if (near_rank(L.near[k], x) < bound) return;
+        const int at = atomicAdd(&L.found[which], 1);
+        if (at < BM_LIST) L.list[which][at] = Pick{x, token, k};
+      });
+    }
+    level_sync<Level>();
+    found = L.found[which];
   }
-  if (found <= BM_LIST || tries > 3) return 0u;
-  return with_margin(L, tighter_bound(L, units, want, Unit::SELF ? BM_LIST : BM_LIST / 8, bound, top, unit));
+  return found;
 }
 
 // The `want` best nodes, and possibly a few more, into L.list[which], in no order; returns how many.
@@ -432,27 +458,19 @@ __device__ __forceinline__ int best_nodes(Level& L, int which, int units, int wa
       }
     }
   };
-  // a node on the list costs the next level a unit; a logit on the last list costs next to nothing
-  const int loose = Unit::SELF ? 3 * want + 64 : BM_LIST;
-  int found, tries = 0;
+  collect(warp, first);
 #pragma unroll 1
-  while (true) {
-    collect(warp, first);
-#pragma unroll 1
-    for (int base = warp + WARPS * AHEAD; base < units; base += WARPS * AHEAD) {
-      Batch b;
-      look(base, b);
-      collect(base, b);
-    }
-    level_sync<Level>();
-    found = L.found[which];
-    if (found <= loose) return found;
-    const unsigned next = next_bound(L, which, units, want, found, tries++, bound, top, unit);
-    if (next <= bound) break;
-    bound = next;
-    if (tid == 0) L.found[which] = 0;
-    level_sync<Level>();
+  for (int base = warp + WARPS * AHEAD; base < units; base += WARPS * AHEAD) {
+    Batch b;
+    look(base, b);
+    collect(base, b);
   }
+  level_sync<Level>();
+  int found = L.found[which];
+  // a node on the list costs the next level a unit; a logit on the last list costs next to nothing
+  const int most = Unit::SELF ? 3 * want + 64 : BM_LIST;
+  if (found <= most) return found;
+  found = fewer_nodes(L, which, units, want, most, found, bound, top, unit);
   if (found <= BM_LIST) return found;
   wait_for_exact<Level>(known);
   one_by_one(L, which, units, want, unit);
