@@ -78,9 +78,11 @@ struct Logprobs {
     if (e != cudaSuccess) return e;
     if (P.top == 0)
       return launch_dependent(given_kernel<FMT>, dim3((rows + LP_THREADS / 32 - 1) / (LP_THREADS / 32)), dim3(LP_THREADS), 0, stream, P);
-    // (72 x 151936 bfloat16, top 20: 23.3 us with 128 threads, 14.8 with 256; 1024 x 32000 float32, top 5: 27.5 and 32.5)
-    return P.top <= BM_FEW ? launch_dependent(logprob_kernel<LP_THREADS, FMT, VEC>, dim3(rows), dim3(LP_THREADS + LP_EXACT), 0, stream, P)
-                           : launch_dependent(logprob_kernel<2 * LP_THREADS, FMT, VEC>, dim3(rows), dim3(2 * LP_THREADS + LP_EXACT), 0, stream, P);
+    // Rows that SMs hold at once wait for loads, and more threads have more of them on their way (512 x 32000
+    // bfloat16, top 5: 13.9 us with 256 threads, 15.4 with 128); of more rows, smaller blocks overlap better
+    // (1024 x 2000, top 5: 21.1 and 12.1).
+    return rows > 4 * 148 ? launch_dependent(logprob_kernel<LP_THREADS, FMT, VEC>, dim3(rows), dim3(LP_THREADS + LP_EXACT), 0, stream, P)
+                          : launch_dependent(logprob_kernel<2 * LP_THREADS, FMT, VEC>, dim3(rows), dim3(2 * LP_THREADS + LP_EXACT), 0, stream, P);
   }
 };
 
