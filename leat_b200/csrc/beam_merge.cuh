@@ -19,7 +19,7 @@ constexpr int BM_MAX_BEAMS = 64;
 constexpr int BM_MAX_WIDTH = 64;
 constexpr int BM_LIST = 512;    // nodes a level hands to the next
 constexpr int BM_PARTS = 128;   // parts of the block whose best bound a level: at least twice the width
-constexpr int BM_FEW = 16;      // up to this width 32 parts, one per lane, will do
+constexpr int BM_FEW = 10;      // up to this width 256 threads go down the levels, 512 beyond
 
 struct MergeParams {
   TileParams T;
