@@ -107,11 +107,14 @@ __device__ __forceinline__ LogSum near_log_sum(TileHead h, TileHead more, const 
   return LogSum{m, (double)log};
 }
 
+// +inf counts as the largest float: the tiles' headers and chunk maxima hold none, and a logit is capped
+// where it is read (a NaN stays one)
+__device__ __forceinline__ float capped(float x) { return x > largest_float() ? largest_float() : x; }
 template <int FMT>
 __device__ __forceinline__ float one_logit(const void* logits, size_t at) {
-  if (FMT == 0) return static_cast<const float*>(logits)[at];
-  if (FMT == 1) return __bfloat162float(static_cast<const __nv_bfloat16*>(logits)[at]);
-  return __half2float(static_cast<const __half*>(logits)[at]);
+  if (FMT == 0) return capped(static_cast<const float*>(logits)[at]);
+  if (FMT == 1) return capped(__bfloat162float(static_cast<const __nv_bfloat16*>(logits)[at]));
+  return capped(__half2float(static_cast<const __half*>(logits)[at]));
 }
 
 // A row's beam: what turns its logits into ranks
@@ -121,9 +124,8 @@ struct Beam {
   float max;       // its largest logit
   int state;       // 0 dead, 1 live, 2 finished
 };
-// +inf counts as the largest float
 __device__ __forceinline__ double score_of(const Beam& b, float x) {
-  return b.base + ((double)fminf(x, largest_float()) - (double)b.max);
+  return b.base + ((double)x - (double)b.max);
 }
 // Ranks to within a margin of themselves and of the beam's reach, scale * (|base| + 8), enough to leave
 // most logits out: 2^-24 each for the rounding of the base, the difference, the sum and the product and
@@ -132,7 +134,8 @@ __device__ __forceinline__ double score_of(const Beam& b, float x) {
 struct __align__(16) Near {
   float base, max, scale, pad;
 };
-// as ordered bits; 0 for what is no continuation: no logit, a NaN, or a beam that is not live
+// as ordered bits; 0 for what is no continuation: no logit, a NaN, or a beam that is not live.  x: at most the
+// largest float; the rank of scores or penalties beyond float32's range is an infinity.
 __device__ __forceinline__ unsigned near_rank(const Near& b, float x) {
   const float v = (b.base + (x - b.max)) * b.scale;
   return x > neg_inf() && v == v ? ord32(v + 0.0f) : 0u;
@@ -244,11 +247,12 @@ __device__ __noinline__ void one_by_one(Level& L, int which, int units, int want
   }
 }
 
-// a near rank's bits less what two of them may be off; 1, which every node reaches, for 0
+// a near rank's bits less what two of them may be off; 1, which every node reaches, for 0 and for an infinity,
+// which says nothing about the ranks behind it (inf - inf would be a NaN, whose bits no node reaches)
 template <typename Level>
 __device__ __forceinline__ unsigned with_margin(const Level& L, unsigned bits) {
   const float b = unord32(bits);
-  return bits > 0u && b > neg_inf() ? ord32(b - L.margin * (fabsf(b) + L.reach) + 0.0f) : 1u;
+  return bits > 0u && fabsf(b) <= largest_float() ? ord32(b - L.margin * (fabsf(b) + L.reach) + 0.0f) : 1u;
 }
 
 // what is on a list, as units (each lane's of its own beam)
@@ -565,7 +569,7 @@ struct VectorUnit {
   __device__ __forceinline__ float peek(int u, int k) const {
     uint32_t w[4];
     load(u, k, w);
-    return largest_of<FMT>(w[0], w[1], w[2], w[3]);
+    return fminf(largest_of<FMT>(w[0], w[1], w[2], w[3]), largest_float());
   }
   template <typename Visit>
   __device__ __forceinline__ void each(int u, int k, Visit&& visit) const {
@@ -573,7 +577,7 @@ struct VectorUnit {
     load(u, k, w);
     const int first = token(u, k);
 #pragma unroll
-    for (int q = 0; q < PER; ++q) visit(held<FMT>(w, q), first + q, q);
+    for (int q = 0; q < PER; ++q) visit(capped(held<FMT>(w, q)), first + q, q);
   }
 };
 

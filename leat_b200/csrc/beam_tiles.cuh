@@ -44,7 +44,7 @@ struct TileParams {
   const float* scores;      // rows whose score is not finite are left out (NULL: none)
   const uint8_t* finished;  // and rows that have finished (NULL: none)
   TileHead* heads;          // (rows, tiles)
-  float* chunk_max;         // (rows, tiles, BT_CHUNKS), in the logits' order
+  float* chunk_max;         // (rows, tiles, BT_CHUNKS), in the logits' order; at most FLT_MAX
 };
 
 __device__ __forceinline__ float largest_float() { return __uint_as_float(0x7F7FFFFFu); }
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(BT_THREADS, 7) beam_tile_kernel(const TilePara
 #pragma unroll
     for (int u = 0; u < BT_VECS; ++u) add_chunk(u);
   }
-  if (lane < BT_VECS) chunk_max[lane * BT_WARPS + warp] = mine;
+  if (lane < BT_VECS) chunk_max[lane * BT_WARPS + warp] = fminf(mine, largest_float());
   M = fminf(M, largest_float());  // the warp's own
   const bool empty = M == neg_inf(), plain = fabsf(M) < PLAIN_LIMIT;
   float s = (part[0] + part[1]) + (part[2] + part[3]);
