@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(BT_THREADS, 7) beam_tile_kernel(const TilePara
 #pragma unroll
     for (int u = 0; u < BT_VECS; ++u) add_chunk(u);
   }
-  if (lane < BT_VECS) chunk_max[lane * BT_WARPS + warp] = fminf(mine, largest_float());
+  if (lane < BT_VECS) chunk_max[lane * BT_WARPS + warp] = mine;
   M = fminf(M, largest_float());  // the warp's own
   const bool empty = M == neg_inf(), plain = fabsf(M) < PLAIN_LIMIT;
   float s = (part[0] + part[1]) + (part[2] + part[3]);
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(BT_THREADS, 7) beam_tile_kernel(const TilePara
   }
   __syncthreads();
   const int cell = row * P.tiles + tile;
-  if (P.with_chunks && tid < BT_CHUNKS) P.chunk_max[(size_t)cell * BT_CHUNKS + tid] = chunk_max[tid];
+  if (P.with_chunks && tid < BT_CHUNKS) P.chunk_max[(size_t)cell * BT_CHUNKS + tid] = fminf(chunk_max[tid], largest_float());
   if (warp == BT_WARPS - 1) {
     const float m = lane < BT_WARPS ? warp_max[lane] : neg_inf();
     const float all = warp_largest(m);
