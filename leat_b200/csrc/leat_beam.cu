@@ -95,14 +95,20 @@ bool logits_fit(const void* logits, int rows, int vocab, long long row_stride, u
 
 int64_t lowest_bit(int64_t x) { return x & -x; }
 
+// Lets a kernel be launched with more shared memory than the 48 KB, some of which it declares, that need no
+// asking.  The limit is the function's, not the call's, so it is always set to the most that any call wants:
+// set to a call's own size, it could be lowered by another thread's call before this one's launch.
+template <typename Kernel>
+cudaError_t allow_shared(Kernel kernel, size_t wanted, int most) {
+  return wanted > 40 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most) : cudaSuccess;
+}
+
 template <int UNIT>
 cudaError_t launch_reorder(const ReorderParams& P, dim3 grid, bool twice, cudaStream_t stream) {
   const size_t shared = (size_t)P.beams * RO_THREADS * column_bytes(twice);
   auto kernel = twice ? reorder_kernel<UNIT, true> : reorder_kernel<UNIT, false>;
-  if (shared > 40 * 1024) {  // (beside what the kernel declares, 48 KB without asking)
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
-    if (e != cudaSuccess) return e;
-  }
+  const cudaError_t e = allow_shared(kernel, shared, (twice ? RO_TWICE_BEAMS : RO_MAX_BEAMS) * RO_THREADS * column_bytes(twice));
+  if (e != cudaSuccess) return e;
   return launch_dependent(kernel, grid, dim3(RO_THREADS), shared, stream, P);
 }
 
@@ -185,7 +191,7 @@ int leat_reorder_states(const leat_state* states, int32_t count, const int32_t* 
   ReorderParams P;
   P.parents = parents; P.slots = slots; P.start = start; P.end = end;
   P.start_all = start_all; P.end_all = end_all; P.beams = beams;
-  const bool twice = beams <= 16;
+  const bool twice = beams <= RO_TWICE_BEAMS;
   const int span = RO_THREADS * column_bytes(twice);  // bytes of a row that a block takes at a time
   // one launch per width of the widest loads that a tensor allows (16, 8, 4, 2, 1 bytes) and 64 of its kind
   for (int unit = 16; unit >= 1; unit /= 2) {
@@ -247,9 +253,7 @@ int leat_beam_sequences(const int32_t* tokens, const int32_t* parents, int32_t s
   const unsigned per_step = (unsigned)(beams / P.vec);
   P.divide = (unsigned)((0x100000000ull + per_step - 1) / per_step);
   const size_t shared = (size_t)9 * chunk * beams;
-  if (shared > 40 * 1024 &&
-      cuda_failed(cudaFuncSetAttribute(sequences_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared), "cudaFuncSetAttribute"))
-    return LEAT_E_CUDA;
+  if (cuda_failed(allow_shared(sequences_kernel, shared, SQ_MOST_SHARED), "cudaFuncSetAttribute")) return LEAT_E_CUDA;
   return cuda_failed(launch_dependent_cluster(blocks, sequences_kernel, dim3((unsigned)(groups * blocks)), dim3(SQ_THREADS), shared, stream, P),
                      "sequences_kernel launch") ? LEAT_E_CUDA : LEAT_OK;
 }

@@ -14,6 +14,7 @@ namespace leat {
 
 constexpr int RO_THREADS = 128;
 constexpr int RO_MAX_BEAMS = 64;
+constexpr int RO_TWICE_BEAMS = 16;  // up to this many, two columns a thread
 constexpr int RO_MAX_STATES = 64;  // tensors per launch: 3 KB of kernel parameters
 
 struct StateRows {  // sizes and strides in bytes

@@ -19,6 +19,7 @@ constexpr int SQ_THREADS = 256;
 constexpr int SQ_MAX_BEAMS = 64;
 constexpr int SQ_MAX_BLOCKS = 8;       // of a cluster
 constexpr int SQ_SHARED = 96 * 1024;   // nine bytes per step and beam: parent, token, path
+constexpr int SQ_MOST_SHARED = SQ_SHARED + 3 * 9 * SQ_MAX_BEAMS;  // (with the steps rounded up to a multiple of four)
 constexpr unsigned SQ_LOST = 255;      // behind a parent out of range: no beam
 
 struct SequenceParams {
