@@ -22,38 +22,47 @@ import torch
 class SlotHistory:
     """ids (slots, capacity) int32 with -1 for unused places (the sampler ignores ids outside the
     vocabulary), count (slots,) int32 of tokens recorded so far; a slot's list is a ring: once
-    `capacity` tokens are in, the oldest are overwritten."""
+    `capacity` tokens are in, the oldest are overwritten.  Slots outside 0..slots-1 (the padding of a batch)
+    are left alone: what is appended to them is dropped, and their history is empty."""
 
     def __init__(self, slots: int, capacity: int, vocab: int, special_ids=(), device=None):
         if slots <= 0 or capacity <= 0 or vocab <= 0:
             raise ValueError("slots, capacity and vocab must be positive")
         self.slots, self.capacity, self.vocab = slots, capacity, vocab
         self.device = torch.device(device) if device is not None else torch.device("cpu")
-        self.ids = torch.full((slots, capacity), -1, dtype=torch.int32, device=self.device)
-        self.count = torch.zeros(slots, dtype=torch.int32, device=self.device)
+        # one row more than slots, always empty, for the slots outside: masking them out of an index would
+        # need its length on the host, and any other row could be one that the same call writes
+        self._ids = torch.full((slots + 1, capacity), -1, dtype=torch.int32, device=self.device)
+        self._count = torch.zeros(slots + 1, dtype=torch.int32, device=self.device)
+        self.ids, self.count = self._ids[:slots], self._count[:slots]
         text = torch.ones(vocab, dtype=torch.bool)
         special = [i for i in special_ids if 0 <= i < vocab]
         if special:
             text[torch.tensor(special, dtype=torch.long)] = False
         self.text = text.to(self.device)  # leat's `_text`: tokens a penalty may lower
 
+    def _rows_of(self, slots: torch.Tensor) -> torch.Tensor:
+        """The rows of `_ids` and `_count` that `slots` are: `self.slots`, the empty one, for those outside."""
+        slots = slots.to(self.device, torch.long).reshape(-1)
+        return slots.clamp(-1, self.slots).remainder(self.slots + 1)
+
     def reset(self, slots: torch.Tensor) -> None:
         """A chunk of prompt empties its slot's tokens (leat/engine.py:772-774)."""
-        slots = slots.to(self.device, torch.long).reshape(-1)
-        self.ids[slots] = -1
-        self.count[slots] = 0
+        rows = self._rows_of(slots)
+        self._ids[rows] = -1
+        self._count[rows] = 0
 
     def append(self, slots: torch.Tensor, tokens: torch.Tensor) -> None:
         """A decode step runs its rows' last tokens and adds each to its slot's (rows with distinct
         slots), unless the token is markup."""
-        slots = slots.to(self.device, torch.long).reshape(-1)
+        rows = self._rows_of(slots)
         tokens = tokens.to(self.device, torch.long).reshape(-1)
-        keep = self.text[tokens.clamp(0, self.vocab - 1)] & (tokens >= 0) & (tokens < self.vocab)
-        count = self.count[slots].to(torch.long)
+        keep = self.text[tokens.clamp(0, self.vocab - 1)] & (tokens >= 0) & (tokens < self.vocab) & (rows < self.slots)
+        count = self._count[rows].to(torch.long)
         place = count % self.capacity
-        old = self.ids[slots, place]
-        self.ids[slots, place] = torch.where(keep, tokens.to(torch.int32), old)
-        self.count[slots] = (count + keep.to(torch.long)).to(torch.int32)
+        old = self._ids[rows, place]
+        self._ids[rows, place] = torch.where(keep, tokens.to(torch.int32), old)
+        self._count[rows] = (count + keep.to(torch.long)).to(torch.int32)
 
     def reorder(self, slots: torch.Tensor, parents: torch.Tensor) -> None:
         """A step of beam search: slots (G, K) are the beams' slots, and slot (g, k) takes the tokens that
@@ -73,17 +82,16 @@ class SlotHistory:
 
     def rows(self, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """(history, history_len) for a decode step over `slots`: what sample() takes."""
-        slots = slots.to(self.device, torch.long).reshape(-1)
-        return self.ids[slots].contiguous(), self.count[slots].clamp(max=self.capacity).contiguous()
+        rows = self._rows_of(slots)
+        return self._ids[rows].contiguous(), self._count[rows].clamp(max=self.capacity).contiguous()
 
     def rows_of_run(self, slots: torch.Tensor, run: torch.Tensor) -> torch.Tensor:
         """History of a speculative step's rows: `run` (n, ran) are the tokens each sequence runs; row
         (i, j) sees its slot's tokens and run tokens 0..j, markup left out.  Returns
         (n * ran, capacity + ran) ids, -1 where nothing is recorded (no lengths needed)."""
-        slots = slots.to(self.device, torch.long).reshape(-1)
         run = run.to(self.device, torch.long)
         n, ran = run.shape
-        base = self.ids[slots].unsqueeze(1).expand(n, ran, self.capacity)
+        base = self._ids[self._rows_of(slots)].unsqueeze(1).expand(n, ran, self.capacity)
         ok = self.text[run.clamp(0, self.vocab - 1)] & (run >= 0) & (run < self.vocab)
         shown = torch.where(ok, run, torch.full_like(run, -1)).to(torch.int32)  # (n, ran)
         upto = torch.tril(torch.ones(ran, ran, dtype=torch.bool, device=self.device))  # row j sees tokens 0..j
