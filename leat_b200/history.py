@@ -77,8 +77,10 @@ class SlotHistory:
             return
         known = (parents >= 0) & (parents < parents.shape[1])
         own = torch.arange(parents.shape[1]).expand_as(parents)
-        to, of = slots.long().reshape(-1), slots.long().gather(1, torch.where(known, parents.long(), own)).reshape(-1)
-        self.ids[to], self.count[to] = self.ids[of], self.count[of]
+        to = self._rows_of(slots).reshape(slots.shape)
+        of = to.gather(1, torch.where(known, parents.long(), own))
+        of = torch.where((to < self.slots) & (of < self.slots), of, to)  # (a slot outside takes nothing and gives nothing)
+        self._ids[to], self._count[to] = self._ids[of], self._count[of]
 
     def rows(self, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """(history, history_len) for a decode step over `slots`: what sample() takes."""

@@ -51,3 +51,17 @@ def test_reset_and_rows():
 def test_shapes_are_the_slots():
     h = SlotHistory(3, 2, 50)
     assert h.ids.shape == (3, 2) and h.count.shape == (3,) and h.ids.is_contiguous() and h.count.is_contiguous()
+
+
+def test_reorder_on_the_cpu_as_on_the_gpu():
+    """A slot outside is no destination, and a beam whose parent's slot is outside keeps its own tokens."""
+    h = _filled(slots=6)
+    ids, count = h.ids.clone(), h.count.clone()
+    slots = torch.tensor([[0, -1, 3], [6, 5, 1], [-1, -1, 1 << 30]])
+    h.reorder(slots, torch.tensor([[2, 0, 1], [1, 2, 0], [1, 0, 0]]))
+    #       0 takes 3's; -1 nothing; 3's parent has no slot; 6 nothing; 5 takes 1's; 1's parent has no slot
+    want = {0: 3, 5: 1}
+    for slot in range(6):
+        of = want.get(slot, slot)
+        assert torch.equal(h.ids[slot], ids[of]) and h.count[slot] == count[of]
+    assert h.rows(torch.tensor([-1, 6]))[1].tolist() == [0, 0]
