@@ -79,8 +79,10 @@ __device__ __forceinline__ LogSum row_log_sum(TileHead h, const TileHead* heads,
   return LogSum{m, plain ? log(s) + ((double)e * ln2_exact - (double)m) - off * (double)m : log(s)};
 }
 
-// the same in float32, to within 2^-19: what the levels below rank by while other warps work out the
-// exact one.  h, more: the lane's headers of the first 64.
+// the same in float32, to within 2^-17: what the levels below rank by while other warps work out the
+// exact one.  h, more: the lane's headers of the first 64.  (Of 2^-17 = 7.6e-6: lg2.approx is good to 2^-22 of
+// a logarithm of up to 31, which is 5.1e-6; that times ln 2, and the sum, are rounded at up to 21.5, 2^-20 or
+// 9.5e-7 each; the lanes' sums are rounded six times, 3.6e-7; the rest is below 2e-7.)
 __device__ __forceinline__ LogSum near_log_sum(TileHead h, TileHead more, const TileHead* heads, int tiles, int lane) {
   constexpr float ln2_float = 0.693147182f, ln2_rest = -1.90465421e-09f, off = -1.3349756e-08f;  // (off: as above)
   if (lane >= tiles) h.max = neg_inf();
@@ -92,12 +94,13 @@ __device__ __forceinline__ LogSum near_log_sum(TileHead h, TileHead more, const 
   const bool plain = fabsf(m) < PLAIN_LIMIT;
   const float e = plain ? ceilf(m * log2e()) : 0.0f;
   auto part = [&](const TileHead& v) {
-    if (!(v.max > neg_inf())) return 0.0f;
-    if (!plain || v.exponent == OVER_MAX) return (float)part_beyond(v, m, plain ? (int)e : OVER_MAX);
-    return (float)(v.sum * two_to(v.exponent - (int)e));
+    if (!(v.max > neg_inf())) return 0.0;
+    if (!plain || v.exponent == OVER_MAX) return part_beyond(v, m, plain ? (int)e : OVER_MAX);
+    return v.sum * two_to(v.exponent - (int)e);
   };
-  float s = part(h) + part(more);
-  for (int t = lane + 64; t < tiles; t += 32) s += part(heads[t]);
+  double sum = part(h) + part(more);
+  for (int t = lane + 64; t < tiles; t += 32) sum += part(heads[t]);
+  float s = (float)sum;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(FULL, s, d);
   float log2_s;
@@ -127,10 +130,14 @@ struct Beam {
 __device__ __forceinline__ double score_of(const Beam& b, float x) {
   return b.base + ((double)x - (double)b.max);
 }
-// Ranks to within a margin of themselves and of the beam's reach, scale * (|base| + 8), enough to leave
-// most logits out: 2^-24 each for the rounding of the base, the difference, the sum and the product and
-// 2^-19 of 1 for the base's own error (so 2^-20 of the reach in all), and with a length penalty 2^-17
-// for the scale's.  A beam that is not live has a NaN for its base.
+// Ranks to within a margin of themselves and of the beam's reach, scale * (|base| + 16), enough to leave most
+// logits out.  The base is off by 2^-17 and its rounding, 2^-24 |base|; the difference x - max, which is at most
+// |base| + |sum|, the sum and the product are rounded, 2^-24 each; the scale is off by 2^-15.4 of itself with a
+// length penalty (near_scale).  In all scale (2^-17 + 2^-23 |base|) + 3 * 2^-24 |rank|, at most 2^-20.6 of the
+// reach and 2^-22.4 of the rank, and 2^-15.4 of the rank with a penalty: twice that, as two ranks are compared,
+// is below MARGIN and below PENALTY_MARGIN.  A beam that is not live has a NaN for its base.
+constexpr float MARGIN = 1.9073486328125e-06f;         // 2^-19
+constexpr float PENALTY_MARGIN = 6.103515625e-05f;     // 2^-14
 struct __align__(16) Near {
   float base, max, scale, pad;
 };
@@ -168,7 +175,7 @@ struct Level {
   float stage[STAGE];  // the tiles' maxima, if they fit
   Beam beams[BM_MAX_BEAMS];
   Near near[BM_MAX_BEAMS];
-  float reach;   // largest scale * (|base| + 8) of the live beams
+  float reach;   // largest scale * (|base| + 16) of the live beams
   float margin;  // how far two near ranks may be off together, relative to theirs and the reach
   Pick list[2][BM_LIST];
   __align__(16) unsigned part_best[BM_PARTS];
@@ -606,7 +613,9 @@ __device__ __noinline__ double length_divisor(int length, float alpha) {
   return pow((5.0 + (double)max(length, 0)) / 6.0, (double)alpha);
 }
 
-// its reciprocal, to within 2^-17 (for 32-bit lengths and |alpha| up to 4; 2^-20 for lengths up to 10^5 and 1)
+// its reciprocal, to within 2^-15.4 of itself for 32-bit lengths and |alpha| up to 4: (5 + length) / 6 is rounded
+// four times (2^-21.5 in its log2), lg2.approx is good to 2^-22 of a logarithm of up to 28.5 (2^-17.2), four times
+// that and the product's rounding at up to 114 (2^-18) make 3.3e-5 in the exponent, times ln 2 2.3e-5
 __device__ __forceinline__ float near_scale(int length, float alpha) {
   float log2_l;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(log2_l) : "f"((5.0f + (float)max(length, 0)) * (1.0f / 6.0f)));
@@ -634,7 +643,7 @@ __global__ void __launch_bounds__(THREADS + BM_EXACT) beam_merge_kernel(const Me
   const int start = start_of(L, P.beams * tiles);
   if (tid == 0) {
     L.reach = 0.0f;
-    L.margin = P.length_penalty == 0.0f ? 1.9073486328125e-06f : 3.0517578125e-05f;  // 2^-19, 2^-15
+    L.margin = P.length_penalty == 0.0f ? MARGIN : PENALTY_MARGIN;
     finished_n = 0;
   }
   __syncthreads();
@@ -675,7 +684,7 @@ __global__ void __launch_bounds__(THREADS + BM_EXACT) beam_merge_kernel(const Me
       const float scale = P.length_penalty == 0.0f ? 1.0f : near_scale(length, P.length_penalty);
       const bool any = sum.max > neg_inf();
       L.near[k] = Near{any ? base : quiet_nan(), sum.max, scale, 0.0f};
-      if (any) atomicMax(reinterpret_cast<int*>(&L.reach), __float_as_int(scale * (fabsf(base) + 8.0f)));
+      if (any) atomicMax(reinterpret_cast<int*>(&L.reach), __float_as_int(scale * (fabsf(base) + 16.0f)));
     }
   }
   level_sync<GroupLevel>();
@@ -767,8 +776,8 @@ __global__ void __launch_bounds__(THREADS + LP_EXACT) logprob_kernel(const Logpr
     const LogSum sum = near_log_sum(heads[min(lane, tiles - 1)], heads[min(lane + 32, tiles - 1)], heads, tiles, lane);
     if (lane == 0) {
       L.near[0] = Near{sum.max > neg_inf() ? -(float)sum.log : quiet_nan(), sum.max, 1.0f, 0.0f};
-      L.reach = fabsf((float)sum.log) + 8.0f;
-      L.margin = 1.9073486328125e-06f;
+      L.reach = fabsf((float)sum.log) + 16.0f;
+      L.margin = MARGIN;
     }
   }
   level_sync<RowLevel>();
