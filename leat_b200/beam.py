@@ -63,6 +63,8 @@ def beam_select(logits, scores: torch.Tensor, width: int | None = None, *, finis
     Masks are the caller's: set a forbidden token's logit to -inf (or the type's lowest value, which
     makes it the last resort).  A row with nothing left has no continuations; a group with too few of
     them has tokens of -1 and scores of -inf in the last places, with their own place as parent.
+    There is no backward pass: logits and scores that a gradient is wanted of are refused (detach them, or
+    call under torch.no_grad()).
     `out`: a Selected of an earlier call (or of your own contiguous tensors) to write into."""
     logits = rows_of_logits(logits)
     dev = logits.device
@@ -72,6 +74,8 @@ def beam_select(logits, scores: torch.Tensor, width: int | None = None, *, finis
     rows, vocab = logits.shape
     if not isinstance(scores, torch.Tensor) or scores.dim() != 2:
         raise ValueError("scores must be a (G, K) float32 tensor")
+    if scores.requires_grad and torch.is_grad_enabled():
+        raise ValueError("no gradient flows through this call: detach the scores, or call under torch.no_grad()")
     shape = scores.shape
     groups, beams = shape
     scores = _whole(scores, torch.float32, shape, dev, "scores")

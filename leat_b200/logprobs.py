@@ -29,6 +29,8 @@ def rows_of_logits(logits) -> torch.Tensor:
     """`logits` as the kernels take it: (B, V) on the device, adjacent logits adjacent in memory."""
     if not isinstance(logits, torch.Tensor):
         logits = device_tensor(logits)
+    elif logits.requires_grad and torch.is_grad_enabled():
+        raise ValueError("no gradient flows through this call: detach the logits, or call under torch.no_grad()")
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in FORMATS or not logits.is_cuda:
         raise ValueError("logits must be a (B, V) float32, bfloat16 or float16 CUDA tensor")
     rows, vocab = logits.shape
@@ -74,8 +76,11 @@ def token_logprobs(logits, ids=None, top: int = 0) -> TokenLogprobs:
     and of each row's `top` likeliest tokens (0..64), with their ids.  logits (B, V) float32, bfloat16
     or float16.  Results are float32, (B, M) and (B, top).
 
-    A NaN logit counts as -inf.  Ids outside the vocabulary (a -1 of padding) and tokens of logit -inf
-    have log-probability -inf, as does everything in a row without a logit above -inf."""
+    There is no backward pass: logits that a gradient is wanted of are refused (detach them, or call under
+    torch.no_grad()).
+
+    A NaN logit counts as -inf, +inf as the largest float.  Ids outside the vocabulary (a -1 of padding) and
+    tokens of logit -inf have log-probability -inf, as does everything in a row without a logit above -inf."""
     logits = rows_of_logits(logits)
     dev = logits.device
     if torch.cuda.current_device() != dev.index:
