@@ -49,8 +49,8 @@ class SlotHistory:
     def reset(self, slots: torch.Tensor) -> None:
         """A chunk of prompt empties its slot's tokens (leat/engine.py:772-774)."""
         rows = self._rows_of(slots)
-        self._ids[rows] = -1
-        self._count[rows] = 0
+        self._ids.index_fill_(0, rows, -1)  # (assigned by index, a number comes from the host: no graph takes that)
+        self._count.index_fill_(0, rows, 0)
 
     def append(self, slots: torch.Tensor, tokens: torch.Tensor) -> None:
         """A decode step runs its rows' last tokens and adds each to its slot's (rows with distinct
