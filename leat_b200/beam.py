@@ -4,7 +4,8 @@ serves requests that ask for the best of several.
 
 `BeamSearch` runs a batch of searches step by step; `beam_select`, `reorder_states` and
 `beam_sequences` are its parts.  Nothing here waits for the device or copies to the host, and a call's
-scratch is its own, so every part can be captured into a CUDA graph."""
+scratch is its own, so every part can be captured into a CUDA graph, and a search as a whole; a single
+step of a `BeamSearch` cannot be captured and replayed for the others (the class says why)."""
 
 from __future__ import annotations
 
@@ -308,7 +309,11 @@ class BeamSearch:
         best = search.sequences()                                 # tokens (G, K, T), best beam first
 
     A step selects the beams' continuations, makes `states` follow their beams (reorder_states), and
-    returns the tokens the beams run next."""
+    returns the tokens the beams run next.
+
+    Steps are counted on the host: the count says which of two sets of beams a step reads and writes, and where
+    its tokens go.  A captured step does that step again whenever it is replayed, so a graph takes a whole
+    search, from reset() to sequences(), or one step of a known number."""
 
     def __init__(self, groups: int, beams: int, max_steps: int, *, end_id: int | None = None, length_penalty: float = 0.0, device=None):
         if groups <= 0 or not 1 <= beams <= MAX_BEAMS or max_steps <= 0:
