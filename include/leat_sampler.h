@@ -292,7 +292,8 @@ int leat_shard_result(leat_shard_t* shard, const leat_sample_args* args, leat_st
    beam's, plus one for a live beam; equal ranks by the lower beam, then the larger logit, then the
    lower token.  Scores and ranks are held in double precision; out_scores is rounded once.  Where a
    group has fewer than `width` continuations the rest read: token -1, score -inf, not finished,
-   length 0, and as parent the beam of the place itself (place % beams). */
+   length 0, and as parent the beam of the place itself (place % beams).  Outputs overlap neither one
+   another nor what is read. */
 typedef struct leat_beam_args {
   const void* logits; /* (groups * beams, vocab): float32, or as LEAT_FLAG_LOGITS_BF16 / _F16 say */
   int32_t groups;

@@ -66,7 +66,8 @@ def beam_select(logits, scores: torch.Tensor, width: int | None = None, *, finis
     them has tokens of -1 and scores of -inf in the last places, with their own place as parent.
     There is no backward pass: logits and scores that a gradient is wanted of are refused (detach them, or
     call under torch.no_grad()).
-    `out`: a Selected of an earlier call (or of your own contiguous tensors) to write into."""
+    `out`: a Selected of an earlier call (or of your own contiguous tensors) to write into; it shares no
+    memory with what the call reads."""
     logits = rows_of_logits(logits)
     dev = logits.device
     if torch.cuda.current_device() != dev.index:
@@ -111,12 +112,19 @@ def beam_select(logits, scores: torch.Tensor, width: int | None = None, *, finis
         wanted = [(out.tokens, torch.int32), (out.parents, torch.int32), (out.scores, torch.float32)]
         wanted += [(out.finished, torch.bool)] if end_id is not None else []
         wanted += [(out.lengths, torch.int32)] if lengths is not None else []
-        read = (scores.data_ptr(), lengths_at, done_at)  # (0 where there is none, as an empty tensor's)
+        # groups write while others still read: the logits (their padding included), the beams', one another's
+        at, scores_at = logits.data_ptr(), scores.data_ptr()
+        taken = [(at, at + ((rows - 1) * logits.stride(0) + vocab) * logits.element_size()), (scores_at, scores_at + 4 * rows),
+                 (lengths_at, lengths_at + 4 * rows), (done_at, done_at + rows)]  # fmt: skip
         for t, dtype in wanted:
             if t is None or t.dtype != dtype or t.shape != (groups, width) or t.device != dev or not t.is_contiguous():
                 raise ValueError(f"out must hold contiguous ({groups}, {width}) tensors on {dev}, of the types of a Selected")
-            if t.data_ptr() in read and groups:
-                raise ValueError("out must not be what the step reads")
+            begin = t.data_ptr()
+            end = begin + groups * width * (1 if dtype == torch.bool else 4)
+            for low, high in taken:
+                if begin < high and low < end:
+                    raise ValueError("out must not be, or overlap, what the step reads or another of its outputs")
+            taken.append((begin, end))
     if groups == 0:
         return out
     if end_id is not None:
