@@ -54,12 +54,18 @@ def _scratch_bytes(rows: int, vocab: int, width: int) -> int:
 # A call's time on the host is most of what a small one takes, so two of torch's inner entry points are
 # used where they are there: the current stream's handle without a Stream object around it (0.1 us for
 # 3.2), and memory of the current device without the keyword arguments' parsing (0.8 us for 1.8).
-raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
-empty_strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
-if empty_strided is None:
+def plain_raw_stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
 
-    def empty_strided(size, stride, dtype):
-        return torch.empty_strided(size, stride, dtype=dtype, device="cuda")
+
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or plain_raw_stream
+
+
+def plain_empty_strided(size, stride, dtype):
+    return torch.empty_strided(size, stride, dtype=dtype, device="cuda")
+
+
+empty_strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None) or plain_empty_strided
 
 
 def scratch(rows: int, vocab: int, width: int) -> tuple[torch.Tensor, int, int]:
