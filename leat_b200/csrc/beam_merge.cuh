@@ -9,7 +9,8 @@
 // The n best are found top down.  A node (a tile of a row, a chunk of a tile, 16 bytes of a chunk) is
 // worth its largest logit's continuation; the n best nodes of a level, in the order above with a
 // node's first token for its token, hold the n best continuations.  So a level is one selection: from
-// all tiles, from the chunks of about n tiles, from the logits of about n chunks.
+// all tiles, from the chunks of about n tiles, from the logits of about n chunks.  Where there are few tiles
+// the first is left out, and the chunks are those of all tiles (start_of).
 #pragma once
 #include "beam_tiles.cuh"
 
@@ -19,7 +20,7 @@ constexpr int BM_MAX_BEAMS = 64;
 constexpr int BM_MAX_WIDTH = 64;
 constexpr int BM_LIST = 512;    // nodes a level hands to the next
 constexpr int BM_PARTS = 128;   // parts of the block whose best bound a level: at least twice the width
-constexpr int BM_FEW = 10;      // up to this width 256 threads go down the levels, 512 beyond
+constexpr int BM_FEW = 10;      // up to this width 256 threads go down the levels, 512 beyond (three parts a place make 30 of 32)
 
 struct MergeParams {
   TileParams T;

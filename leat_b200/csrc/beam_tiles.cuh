@@ -8,7 +8,7 @@
 // multiply-add, an ex2 and an addition.
 //
 // Nothing is selected here.  What leaves a block is a header (maximum, sum) and the maximum of each of
-// the tile's 32 chunks of adjacent logits: 1 % of what was read.  The n largest of any set of nodes
+// the tile's 32 chunks of adjacent logits: 144 bytes of 16 KB read, 0.9 %.  The n largest of any set of nodes
 // hold the n largest logits below them, so a handful of tiles, of their chunks and of the chunks'
 // logits are all that the few blocks after this pass look at (beam_merge.cuh).
 #pragma once

@@ -40,8 +40,8 @@ bool known_format(uint32_t flags) {
          flags != (uint32_t)(LEAT_FLAG_LOGITS_BF16 | LEAT_FLAG_LOGITS_F16);
 }
 
-// whole 16-byte vectors where the rows allow it, one logit per load elsewhere: the same for every row
-// of a call, so that equal rows have equal sums
+// Whole 16-byte vectors where the rows allow it; elsewhere float32 logits one per load, and 16-bit ones in
+// whole vectors that are shifted.  It is the same for every row of a call, so that equal rows have equal sums.
 template <template <int, bool> class Launch, typename Params>
 cudaError_t by_format(const Params& P, uint32_t flags, int rows, int blocks, cudaStream_t stream) {
   const TileParams& T = P.T;
@@ -66,9 +66,14 @@ struct Select {
   static cudaError_t both(const MergeParams& P, int rows, int groups, cudaStream_t stream) {
     const cudaError_t e = Tiles<FMT, VEC>::launch(P.T, rows, stream);
     if (e != cudaSuccess) return e;
-    // few continuations: small blocks, whose barriers and bounds cost less; many: more nodes at a time (80 x
-    // 151936 bfloat16 in 16 groups with 256 and 512 threads, us: width 4 12.9 and 13.1, 10 14.0 and 13.4, 16
-    // 15.8 and 14.1, 64 38 and 26; 256 x 262144 float32: width 8 48.1 and 48.9, 10 49.9 and 51.6, 64 78 and 65)
+    // Many continuations: more threads, for more nodes at a time.  Few: small blocks, whose barriers and bounds
+    // cost less.  The border is the width up to which a level may bound itself by 32 parts, which wants few
+    // warps to have many units each.  With 256 and 512 threads, us in a captured graph, inputs from memory:
+    //   80 x 151936 bfloat16 in 16 groups: width 4 14.3 and 14.5, 10 15.6 and 14.8, 16 17.4 and 15.4, 64 41 and 27
+    //   256 x 262144 float32 in 32 groups: 8 48.7 and 49.4, 10 50.3 and 52.2, 16 49.9 and 49.7, 64 79 and 65
+    //   256 x 32000 bfloat16 in 64 groups: 8 12.4 and 12.5, 10 12.6 and 15.5, 12 13.0 and 12.6, 64 36 and 28
+    //   one group of 4 x 128256: float32 8 8.9 and 10.0, 10 9.0 and 9.7; bfloat16 8 9.6 and 8.3, 10 9.9 and 8.4
+    // (so neither is always better below it; beyond 16, 512 is)
     return P.width <= BM_FEW ? launch_dependent(beam_merge_kernel<256, FMT, VEC>, dim3(groups), dim3(256 + BM_EXACT), 0, stream, P)
                              : launch_dependent(beam_merge_kernel<512, FMT, VEC>, dim3(groups), dim3(512 + BM_EXACT), 0, stream, P);
   }
