@@ -290,7 +290,8 @@ int leat_shard_result(leat_shard_t* shard, const leat_sample_args* args, leat_st
    is dead and continues with nothing.  The logits of finished and dead beams are not read.
    Continuations are ranked by score / ((5 + length) / 6)^length_penalty, where length is the
    beam's, plus one for a live beam; equal ranks by the lower beam, then the larger logit, then the
-   lower token.  Scores and ranks are held in double precision; out_scores is rounded once.  Where a
+   lower token.  Scores and ranks are held in double precision; out_scores is rounded once (a score
+   beyond float's range to -inf).  Where a
    group has fewer than `width` continuations the rest read: token -1, score -inf, not finished,
    length 0, and as parent the beam of the place itself (place % beams).  Outputs overlap neither one
    another nor what is read. */

@@ -139,13 +139,16 @@ __device__ __forceinline__ double score_of(const Beam& b, float x) {
 // is below MARGIN and below PENALTY_MARGIN.  A beam that is not live has a NaN for its base.
 constexpr float MARGIN = 1.9073486328125e-06f;         // 2^-19
 constexpr float PENALTY_MARGIN = 6.103515625e-05f;     // 2^-14
+// All of it is held as a quarter of itself: the lowest value below the largest float, and a score of as much
+// again, stay in range (as infinities they would be below everything, whatever their beams' penalties).
 struct __align__(16) Near {
-  float base, max, scale, pad;
+  float base, max, scale, pad;  // quarters of the base and the maximum
 };
+constexpr float NEAR_UNIT = 0.25f;
 // as ordered bits; 0 for what is no continuation: no logit, a NaN, or a beam that is not live.  x: at most the
-// largest float; the rank of scores or penalties beyond float32's range is an infinity.
+// largest float; a rank that its penalty takes out of float32's range is an infinity.
 __device__ __forceinline__ unsigned near_rank(const Near& b, float x) {
-  const float v = (b.base + (x - b.max)) * b.scale;
+  const float v = (b.base + __fmaf_rn(x, NEAR_UNIT, -b.max)) * b.scale;
   return x > neg_inf() && v == v ? ord32(v + 0.0f) : 0u;
 }
 
@@ -176,7 +179,7 @@ struct Level {
   float stage[STAGE];  // the tiles' maxima, if they fit
   Beam beams[BM_MAX_BEAMS];
   Near near[BM_MAX_BEAMS];
-  float reach;   // largest scale * (|base| + 16) of the live beams
+  float reach;   // largest scale * (|base| + 16) of the live beams, a quarter of it
   float margin;  // how far two near ranks may be off together, relative to theirs and the reach
   Pick list[2][BM_LIST];
   __align__(16) unsigned part_best[BM_PARTS];
@@ -684,8 +687,8 @@ __global__ void __launch_bounds__(THREADS + BM_EXACT) beam_merge_kernel(const Me
       const float base = score - (float)sum.log;
       const float scale = P.length_penalty == 0.0f ? 1.0f : near_scale(length, P.length_penalty);
       const bool any = sum.max > neg_inf();
-      L.near[k] = Near{any ? base : quiet_nan(), sum.max, scale, 0.0f};
-      if (any) atomicMax(reinterpret_cast<int*>(&L.reach), __float_as_int(scale * (fabsf(base) + 16.0f)));
+      L.near[k] = Near{any ? base * NEAR_UNIT : quiet_nan(), sum.max * NEAR_UNIT, scale, 0.0f};
+      if (any) atomicMax(reinterpret_cast<int*>(&L.reach), __float_as_int(scale * ((fabsf(base) + 16.0f) * NEAR_UNIT)));
     }
   }
   level_sync<GroupLevel>();
@@ -776,8 +779,8 @@ __global__ void __launch_bounds__(THREADS + LP_EXACT) logprob_kernel(const Logpr
   if (tid < 32) {
     const LogSum sum = near_log_sum(heads[min(lane, tiles - 1)], heads[min(lane + 32, tiles - 1)], heads, tiles, lane);
     if (lane == 0) {
-      L.near[0] = Near{sum.max > neg_inf() ? -(float)sum.log : quiet_nan(), sum.max, 1.0f, 0.0f};
-      L.reach = fabsf((float)sum.log) + 16.0f;
+      L.near[0] = Near{sum.max > neg_inf() ? -(float)sum.log * NEAR_UNIT : quiet_nan(), sum.max * NEAR_UNIT, 1.0f, 0.0f};
+      L.reach = (fabsf((float)sum.log) + 16.0f) * NEAR_UNIT;
       L.margin = MARGIN;
     }
   }
