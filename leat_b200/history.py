@@ -34,12 +34,27 @@ class SlotHistory:
         # need its length on the host, and any other row could be one that the same call writes
         self._ids = torch.full((slots + 1, capacity), -1, dtype=torch.int32, device=self.device)
         self._count = torch.zeros(slots + 1, dtype=torch.int32, device=self.device)
-        self.ids, self.count = self._ids[:slots], self._count[:slots]
         text = torch.ones(vocab, dtype=torch.bool)
         special = [i for i in special_ids if 0 <= i < vocab]
         if special:
             text[torch.tensor(special, dtype=torch.long)] = False
         self.text = text.to(self.device)  # leat's `_text`: tokens a penalty may lower
+
+    @property
+    def ids(self) -> torch.Tensor:
+        return self._ids[: self.slots]
+
+    @ids.setter
+    def ids(self, ids: torch.Tensor) -> None:
+        self._ids[: self.slots] = ids
+
+    @property
+    def count(self) -> torch.Tensor:
+        return self._count[: self.slots]
+
+    @count.setter
+    def count(self, count: torch.Tensor) -> None:
+        self._count[: self.slots] = count
 
     def _rows_of(self, slots: torch.Tensor) -> torch.Tensor:
         """The rows of `_ids` and `_count` that `slots` are: `self.slots`, the empty one, for those outside."""

@@ -65,3 +65,16 @@ def test_reorder_on_the_cpu_as_on_the_gpu():
         of = want.get(slot, slot)
         assert torch.equal(h.ids[slot], ids[of]) and h.count[slot] == count[of]
     assert h.rows(torch.tensor([-1, 6]))[1].tolist() == [0, 0]
+
+
+def test_copies_and_assigned_tensors_work_on():
+    import copy
+    import pickle
+
+    for other in (lambda h: h, copy.copy, copy.deepcopy, lambda h: pickle.loads(pickle.dumps(h))):
+        h = other(SlotHistory(3, 2, 50))
+        h.append(torch.tensor([1]), torch.tensor([4]))
+        assert h.ids.tolist() == [[-1, -1], [4, -1], [-1, -1]] and h.count.tolist() == [0, 1, 0]
+        h.ids, h.count = torch.tensor([[7, 8], [9, -1], [-1, -1]], dtype=torch.int32), torch.tensor([2, 1, 0], dtype=torch.int32)
+        h.append(torch.tensor([1, -1]), torch.tensor([5, 6]))
+        assert h.ids.tolist() == [[7, 8], [9, 5], [-1, -1]] and h.rows(torch.tensor([1, -1]))[1].tolist() == [2, 0]
